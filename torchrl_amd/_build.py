@@ -26,7 +26,11 @@ SOURCES = ['trl_host.cpp', 'trl_replay.hip', 'trl_gae.hip', 'trl_loss.hip', 'trl
 HEADERS = [os.path.join(CSRC, 'trl_common.h'), os.path.join(ROOT, 'include', 'trl_hip.h')]
 
 # -ffp-contract=off: the parity bar is the reference's op order, one f32 rounding per op.
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (hipcc forms them from ordinary float code; some of their forms have given
+# wrong values now and then on this hardware).  The arithmetic is the same, one instruction per element; the host pass
+# does not know the feature and says so: harmless.
 FLAGS = ['-O3', '-std=c++17', '--offload-arch=gfx950', '-fPIC', '-ffp-contract=off',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
          '-fno-gpu-rdc', '-Wall', '-Wno-unused-function']
 
 

@@ -243,7 +243,7 @@ __device__ __forceinline__ float row_sum16(float x) {
 //     quotient is far from overflow, and a quotient in the subnormal range is added to a parameter.
 // Correctly rounded quotients are unique, so in the ranges above these are the bits of __fdiv_rn
 // (tests/test_gpu_epoch.py::test_fast_adam_is_trl_adam_elem_bit_for_bit, on the diagnostic build).  Written on 4-vectors:
-// the multiplies, adds and fmas pair up as v_pk_*_f32.  clip = +inf means none (med3 then returns the gradient).
+// one 16 B load or store per four elements.  clip = +inf means none (med3 then returns the gradient).
 struct AdamV {
   float w1, beta2, c2, eps, clip, c, rc, neg_step;
 };

@@ -240,7 +240,7 @@ __device__ __forceinline__ void fwd_layer1(f32x16 (&h2)[2], const f32x16 (&h1)[2
 }
 
 // last layer on the VALU: out[n] = WL[n] . hl + bL[n] (both lane halves end with the row's value).  Two features
-// at a time (v_pk_fma_f32: a register pair of the activations times a pair of the 16 B weight read);
+// at a time (a register pair of the activations times a pair of the 16 B weight read);
 // p[n] = (sum over even registers, sum over odd registers)
 template <int NO>
 __device__ __forceinline__ void fwd_last_acc(f32x2 (&p)[NO], const f32x16 (&hl)[2], const float *sWL, int half) {
@@ -1135,7 +1135,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 #pragma unroll
         for (int n = 0; n < NO; ++n) wlb[n] = NO == 1 ? 0.f : sWL[wl_off + (q * NO + n) * 64 + nb * 32 + r32];
         // two rows at a time: the pair (r, r + 1) is a register pair of the product and of the 16 B reads, so the
-        // FMAs are v_pk_fma_f32 (two per instruction, no moves); sums of even and odd rows are kept apart
+        // FMAs need no moves; sums of even and odd rows are kept apart
         f32x2 sdb = {0.f, 0.f};
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
@@ -1495,7 +1495,7 @@ __global__ __launch_bounds__(512) void k_ac_learn_pair(LearnArgs P) {
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          f32x2 t0 = {0.f, 0.f}, t1 = {0.f, 0.f};      // (two features per v_pk_fma_f32)
+          f32x2 t0 = {0.f, 0.f}, t1 = {0.f, 0.f};      // (two features at a time)
 #pragma unroll
           for (int n = 0; n < NO; ++n) {
             const float4 w4 = *(const float4 *)(sWL + n * 64 + kb * 32 + 8 * q + 4 * half);
@@ -2050,7 +2050,7 @@ __global__ __launch_bounds__(512) void k_ac_learn_pair_bx(LearnArgs P) {
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          f32x2 t0 = {0.f, 0.f}, t1 = {0.f, 0.f};      // (two features per v_pk_fma_f32)
+          f32x2 t0 = {0.f, 0.f}, t1 = {0.f, 0.f};      // (two features at a time)
 #pragma unroll
           for (int n = 0; n < NO; ++n) {
             const float4 w4 = *(const float4 *)(sWL + n * 64 + kb * 32 + 8 * q + 4 * half);
