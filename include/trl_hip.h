@@ -51,6 +51,9 @@ extern "C" {
 /* storage dtype of a replay column / output dtype of a gathered column */
 #define TRL_F32 0
 #define TRL_U8 1
+/* further element types of the layer kernels (layer norm, dropout, decay attention) */
+#define TRL_BF16 2
+#define TRL_F16 3
 
 /* GAE modes */
 #define TRL_GAE_REFERENCE 0 /* done ignored inside the trajectory (reference behaviour) */
@@ -612,6 +615,58 @@ int trl_act_categorical(const float *probs, int64_t n, int32_t A, uint64_t seed,
 int trl_act_ou_noise(const float *actor_out, int64_t n, int32_t A, const float *state_in, float *state_out, double theta,
                      double mu, double sigma, double low, double high, uint64_t seed, uint64_t call, float *actions,
                      void *stream);
+
+/* ------------------------------------------------------------------ layer norm, dropout
+ * The normalising and the regularising layer of a Linear / ReLU stack.  No counterpart in the reference (its stacks are
+ * Linear + ReLU, models.py:6-147).  x, y, gy, dx: dense [rows, width] of `dtype` (TRL_F32, TRL_BF16, TRL_F16), any alignment
+ * of the element; weight, bias, mean, rstd and their gradients f32.  1 <= width < 2^24, rows * width < 2^40; rows may be 0.
+ *
+ * fwd: y = (x - m) r * weight + bias per row, m = mean, r = 1 / sqrt(variance + eps), act = 1: max(y, 0) (a NaN stays one).
+ *   weight / bias NULL: ones / zeros.  mean, rstd [rows] (NULL: not written) are what bwd takes.
+ * bwd: any of dx, dweight, dbias may be NULL.  `workspace`: trl_layer_norm_bwd_workspace_bytes bytes, free for other use once
+ *   the call's work is done (not needed when dweight and dbias are NULL).  Sums run in a fixed order: the same bits every run. */
+int trl_layer_norm_fwd(const void *x, const float *weight, const float *bias, int64_t rows, int64_t width, int32_t dtype,
+                       double eps, int32_t act, void *y, float *mean, float *rstd, void *stream);
+int64_t trl_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width, int32_t dtype);
+int trl_layer_norm_bwd(const void *gy, const void *x, const float *weight, const float *bias, const float *mean,
+                       const float *rstd, int64_t rows, int64_t width, int32_t dtype, int32_t act, void *dx, float *dweight,
+                       float *dbias, void *workspace, void *stream);
+
+/* y[i] = (residual ? residual[i] : 0) + (kept(i) ? x[i] / (1 - p) : 0) over n elements (n < 2^40), 0 <= p < 1.  Element i is
+ * kept when word i % 4 of Philox-4x32-10 -- key = seed, counter = (call low, call high, (i / 4) low, (i / 4) high | 2^31) --
+ * is at least round(p 2^32); no mask is stored, the gradient of x is the same call on dL/dy (residual NULL).  `call` is read
+ * from *call_d (device) when that is not NULL: a captured graph then draws a new mask at every replay. */
+int trl_dropout(const void *x, const void *residual, int64_t n, int32_t dtype, double p, uint64_t seed, uint64_t call,
+                const int64_t *call_d, void *y, void *stream);
+/* *call = (*counter)++ (device, atomic): numbers the calls of a captured graph, or of several streams. */
+int trl_next_call(int64_t *counter, int64_t *call, void *stream);
+
+/* ------------------------------------------------------------------ decay attention
+ * Linear attention with a decay per head over a rollout, no counterpart in the reference.  For env n and head h:
+ *   S_t = (start_t ? 0 : decay[h] * S_{t-1}) + k_t v_t^T,   out_t = scale * q_t^T S_t      for t < lengths[n],
+ * S_{-1} = state_in (NULL: zeros), state_out = S after the sequence's last step (state_in itself where its length is 0);
+ * out is zero at and past lengths[n], where q, k, v and start are not read.  q, k: [T, N, H, dk], v: [T, N, H, dv] of `dtype`
+ * with strides[9] = (t, n, h) of q, of k and of v in elements (a dimension may have stride 0; the last one is dense);
+ * out [T, N, H, dv] dense; states [N, H, dk, dv] f32 dense; decay [H] f32, each in [0, 1]; start [T, N] dense, start_dtype
+ * TRL_F32 or TRL_U8, not zero = the step does not see the ones before it; lengths [N] int32, cut to [0, T], or NULL.
+ * 1 <= dk, dv <= 128, T < 2^30, N * H < 2^22.  Sums and states in f32.
+ * bwd: gy [T, N, H, dv] dense, gstate (gradient of state_out) [N, H, dk, dv] or NULL; dq, dk_out, dv_out dense; dstate
+ *   (gradient of state_in) or NULL.  Zero at and past lengths[n].
+ * step: the same for one step, q, k [N, H, dk], v [N, H, dv], start [N]; state_out may be state_in.
+ * workspace: trl_decay_attention_workspace_bytes bytes (0: none needed), for the calls that split time. */
+int64_t trl_decay_attention_workspace_bytes(int64_t T, int64_t N, int32_t H, int32_t dk, int32_t dv, int32_t backward);
+int trl_decay_attention_fwd(const void *q, const void *k, const void *v, const int64_t *strides, const float *decay,
+                            const void *start, int32_t start_dtype, const int32_t *lengths, const float *state_in, int64_t T,
+                            int64_t N, int32_t H, int32_t dk, int32_t dv, int32_t dtype, double scale, void *out,
+                            float *state_out, void *workspace, void *stream);
+int trl_decay_attention_bwd(const void *gy, const float *gstate, const void *q, const void *k, const void *v,
+                            const int64_t *strides, const float *decay, const void *start, int32_t start_dtype,
+                            const int32_t *lengths, const float *state_in, int64_t T, int64_t N, int32_t H, int32_t dk,
+                            int32_t dv, int32_t dtype, double scale, void *dq, void *dk_out, void *dv_out, float *dstate,
+                            void *workspace, void *stream);
+int trl_decay_attention_step(const void *q, const void *k, const void *v, const float *decay, const void *start,
+                             int32_t start_dtype, const float *state_in, int64_t N, int32_t H, int32_t dk, int32_t dv,
+                             int32_t dtype, double scale, void *out, float *state_out, void *stream);
 
 /* ------------------------------------------------------------------ no-allocation entry point
  * trl_ppo_loss for callers that cannot allocate or bring a workspace: code under HIP graph capture, tight serving

@@ -14,7 +14,7 @@ if os.environ.get('TRL_LIB') == 'tune':
   LIB_PATH = os.path.join(_PKG, 'lib', 'libtrl_hip_tune.so')
 
 TRL_MAX_COLS = 8
-TRL_F32, TRL_U8 = 0, 1
+TRL_F32, TRL_U8, TRL_BF16, TRL_F16 = 0, 1, 2, 3
 TRL_GAE_REFERENCE, TRL_GAE_MASKED = 0, 1
 TRL_LAYOUT_TN, TRL_LAYOUT_NT, TRL_LAYOUT_BLOCKED = 0, 1, 2
 TRL_LOSS_MSE, TRL_LOSS_HUBER = 0, 1
@@ -146,6 +146,17 @@ PROTOTYPES = {
                                               _i64, _f64, _i32, _i32, _f64, _vp, C.POINTER(AdamArgs), _vp, _vp]),
     'trl_dqn_learn_fused_u8': (C.c_int, [C.POINTER(MlpDesc)] * 2 + [_vp] * 5 + [_i64, _f64, _i32, _i32, _f64, _vp,
                                       C.POINTER(AdamArgs), _vp, _vp]),
+    'trl_layer_norm_fwd': (C.c_int, [_vp, _vp, _vp, _i64, _i64, _i32, _f64, _i32, _vp, _vp, _vp, _vp]),
+    'trl_layer_norm_bwd_workspace_bytes': (_i64, [_i64, _i64, _i32]),
+    'trl_layer_norm_bwd': (C.c_int, [_vp] * 6 + [_i64, _i64, _i32, _i32] + [_vp] * 5),
+    'trl_dropout': (C.c_int, [_vp, _vp, _i64, _i32, _f64, C.c_uint64, C.c_uint64, _vp, _vp, _vp]),
+    'trl_next_call': (C.c_int, [_vp, _vp, _vp]),
+    'trl_decay_attention_workspace_bytes': (_i64, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    'trl_decay_attention_fwd': (C.c_int, [_vp] * 3 + [C.POINTER(_i64), _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i32, _i32, _i32,
+                                          _i32, _f64] + [_vp] * 4),
+    'trl_decay_attention_bwd': (C.c_int, [_vp] * 5 + [C.POINTER(_i64), _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i32, _i32, _i32,
+                                          _i32, _f64] + [_vp] * 6),
+    'trl_decay_attention_step': (C.c_int, [_vp] * 5 + [_i32, _vp, _i64, _i32, _i32, _i32, _i32, _f64] + [_vp] * 3),
 }
 
 _lib = None

@@ -56,7 +56,8 @@ class DDPGController(Controller):
                action_low, action_high,
                actor_lr=1e-4, critic_lr=1e-3, gamma=0.99,
                tau=1e-2, n_reset_interval=100, device=None,
-               hidden=256, huber_delta=None, process_group=None, graph=False, fused=None):
+               hidden=256, huber_delta=None, process_group=None, graph=False, fused=None,
+               layer_norm=False, dropout=0.0):
     self.device = resolve_device(device)
     self.action_low = action_low
     self.action_high = action_high
@@ -67,8 +68,8 @@ class DDPGController(Controller):
     self._actor, self._target_actor = FlatParams(self.actor, fresh_grads=True), FlatParams(self.target_actor)
     self._target_actor.copy_from(self._actor)
 
-    self.critic = DDPGCriticNet(obs_size, action_size, hidden).to(self.device)
-    self.target_critic = DDPGCriticNet(obs_size, action_size, hidden).to(self.device)
+    self.critic = DDPGCriticNet(obs_size, action_size, hidden, layer_norm, dropout).to(self.device)
+    self.target_critic = DDPGCriticNet(obs_size, action_size, hidden, layer_norm, dropout).to(self.device)
     self._critic, self._target_critic = FlatParams(self.critic, fresh_grads=True), FlatParams(self.target_critic)
     self._target_critic.copy_from(self._critic)
 
@@ -76,14 +77,16 @@ class DDPGController(Controller):
     self._sync.broadcast_params(self._actor, self._target_actor, self._critic, self._target_critic)
     self.actor_optim = FlatAdam(self._actor, lr=actor_lr, grad_scale=self._sync.scale, device_state=graph)
     self.critic_optim = FlatAdam(self._critic, lr=critic_lr, grad_scale=self._sync.scale, device_state=graph)
+    # (buffers: dropout's call counters, so that a graph's warm-up leaves them as they were)
     self._run = LearnRunner(self._learn_body, [self.actor_optim, self.critic_optim],
-                            lambda: [self._target_actor.data, self._target_critic.data], self.device,
+                            lambda: [self._target_actor.data, self._target_critic.data,
+                                     *self.critic.buffers(), *self.target_critic.buffers()], self.device,
                             graph and not self._sync.enabled)
 
     # the whole step as 10 phases in one launch, or 10 launches (csrc/trl_offpolicy.hip) for two-hidden-layer stacks (eager, or captured once and replayed with graph=True: the Adam step counts then live on the device);
     # config.fused_learn = False / fused=False keeps the autograd path
     self._fused = None
-    if self.device.type == 'cuda' and (config.fused_learn if fused is None else fused):
+    if self.device.type == 'cuda' and (config.fused_learn if fused is None else fused) and not (layer_norm or dropout):
       lins = [[m for m in net.net if isinstance(m, torch.nn.Linear)]
               for net in (self.actor, self.critic, self.target_actor, self.target_critic)]
       if F.FusedDdpgLearn.supports(*lins):

@@ -37,12 +37,13 @@ class DQNController(Controller):
                double_dqn=False, gamma=.99, lr=1e-3,
                eps_max=1.0, eps_min=1e-2, n_eps_anneal=1000,
                n_update_interval=5, device=None,
-               huber_delta=None, hidden=128, process_group=None, graph=False, fused=None):
+               huber_delta=None, hidden=128, process_group=None, graph=False, fused=None,
+               layer_norm=False, dropout=0.0):
     self.action_size = action_size
     self.device = resolve_device(device)
 
-    self.q_net = QNet(obs_size, action_size, hidden).to(self.device)
-    self.target_q_net = QNet(obs_size, action_size, hidden).to(self.device)
+    self.q_net = QNet(obs_size, action_size, hidden, layer_norm, dropout).to(self.device)
+    self.target_q_net = QNet(obs_size, action_size, hidden, layer_norm, dropout).to(self.device)
     # stacks the whole-network kernels take (<= 64 wide) get their gradients written in place by the
     # fused backward; the reference's 128-wide QNet goes through autograd, where fresh gradient
     # tensors + one multi-tensor copy replace a fill and six accumulate launches per step
@@ -58,12 +59,15 @@ class DQNController(Controller):
     self.q_net_optim = FlatAdam(self._q, lr=lr, grad_scale=self._sync.scale, device_state=graph)
     if fusable:     # one use per backward, zeroed grads: let the fused backward write .grad itself
       self.q_net.net.direct_grads = True
-    self._run = LearnRunner(self._learn_body, [self.q_net_optim], lambda: [], self.device, graph)
+    self._dropout = dropout > 0
+    # (dropout's call counters: a graph's warm-up leaves them as they were)
+    buffers = lambda: [b for net in (self.q_net, self.target_q_net) for b in net.buffers()]
+    self._run = LearnRunner(self._learn_body, [self.q_net_optim], buffers, self.device, graph)
 
     # the step up to Adam as 6 launches (csrc/trl_offpolicy.hip) for two-hidden-layer Q-networks up
     # to 1024 wide / fan-in (any fan-in for uint8 frames), eager or graph-replayed; config.fused_learn = False / fused=False keeps the autograd path
     self._fused = None
-    if self.device.type == 'cuda' and (config.fused_learn if fused is None else fused):
+    if self.device.type == 'cuda' and (config.fused_learn if fused is None else fused) and not (layer_norm or dropout):
       lins = [[m for m in net.net if isinstance(m, torch.nn.Linear)] for net in (self.q_net, self.target_q_net)]
       if F.FusedDqnLearn.supports(*lins):
         self._fused = F.FusedDqnLearn(*lins, self._q, self._target)
@@ -77,6 +81,8 @@ class DQNController(Controller):
     self._act_rng = F.ActRng()
 
   def act(self, obs):
+    if self._dropout:
+      self.q_net.eval()      # (learn() switches back)
     with torch.no_grad():
       greedy = self.q_net(obs_to_tensor(obs, self.device)).argmax(dim=-1).cpu().numpy()
     actions = epsilon_greedy(self.action_size, greedy, self.eps.value)
@@ -89,6 +95,8 @@ class DQNController(Controller):
     themselves differ because the reference uses numpy's global generator on the host."""
     need_hip(self.device, 'DQNController.act_device')
     obs = obs_to_tensor(obs, self.device)
+    if self._dropout:
+      self.q_net.eval()      # (learn() switches back)
     with torch.no_grad():
       q = self.q_net(obs)
     return F.act_epsilon_greedy(q, self.eps.value, self._act_rng)      # one launch (csrc/trl_act.hip)

@@ -81,6 +81,45 @@ class SkinnyLinear(nn.Linear):
     return super().forward(x)
 
 
+class LayerNorm(nn.LayerNorm):
+  """nn.LayerNorm over the last dimension (same parameters, same values) on the HIP layer (csrc/trl_norm.hip) for device
+  batches; `relu=True` applies the ReLU behind it in the same launch.  CPU tensors and config.fused_mlp = False take torch's."""
+
+  def __init__(self, width, eps=1e-5):
+    super().__init__(int(width), eps=eps)
+
+  def forward(self, x, relu=False):
+    if x.is_cuda and _fused_mlp_enabled():
+      return _F.layer_norm(x, self.weight, self.bias, self.eps, relu=relu)
+    x = super().forward(x)
+    return torch.relu(x) if relu else x
+
+
+class Dropout(nn.Module):
+  """Dropout with an optional residual, y = residual + dropout(x), whose masks are functions of (seed, call number,
+  element) and are never stored (csrc/trl_norm.hip).  The call number is a device buffer that every training call draws
+  from and raises on the stream, so a step captured into a HIP graph gets a new mask at every replay, and a checkpoint
+  carries on where it was taken.  seed: by default torch.initial_seed() mixed with a number that differs for every layer of
+  the process and every rank.  In eval mode x passes through."""
+
+  def __init__(self, p, seed=None):
+    super().__init__()
+    if not 0.0 <= p < 1.0:
+      raise ValueError('Dropout: p must be in [0, 1), got %r' % (p,))
+    self.p = float(p)
+    self._rng = _F.ActRng(seed)
+    self.register_buffer('calls', torch.zeros(1, dtype=torch.int64))
+
+  def forward(self, x, residual=None):
+    if not self.training or self.p == 0.0:
+      return x if residual is None else residual + x
+    seed, _ = self._rng.next()
+    return _F.dropout(x, self.p, seed, _F.next_call(self.calls), residual=residual)
+
+  def extra_repr(self):
+    return 'p=%g' % self.p
+
+
 def _as_sizes(hidden, depth):
   """int -> `depth` hidden layers of that width; tuple/list -> as given."""
   if isinstance(hidden, (tuple, list)):
@@ -113,6 +152,9 @@ class _Mlp(nn.Sequential):
       if type(m) in (nn.Linear, SkinnyLinear) and m.bias is not None and i + 1 < len(mods) and \
           isinstance(mods[i + 1], nn.ReLU):
         x = _LinearReluFn.apply(x, m.weight, m.bias)
+        i += 2
+      elif _norm_relu(mods, i):
+        x = m(x, relu=True)
         i += 2
       else:
         x = m(x)
@@ -152,10 +194,18 @@ class _Mlp(nn.Sequential):
         relu = i + 1 < len(mods) and isinstance(mods[i + 1], nn.ReLU)
         x = _F.linear_act(x, m.weight, m.bias, relu=relu)
         i += 2 if relu else 1
+      elif _norm_relu(mods, i):
+        x = m(x, relu=True)
+        i += 2
       else:
         x = m(x)
         i += 1
     return x
+
+
+def _norm_relu(mods, i):
+  """A LayerNorm with a ReLU right behind it: one launch."""
+  return isinstance(mods[i], LayerNorm) and i + 1 < len(mods) and isinstance(mods[i + 1], nn.ReLU)
 
 
 def _fusable_stack(mods):
@@ -228,11 +278,17 @@ def _fused_mlp_enabled():
   return config.fused_mlp
 
 
-def _mlp(n_in, hidden_sizes, n_out, tail=None):
-  """Linear/ReLU stack whose Linear layers sit at even Sequential indices (0, 2, 4, ...)."""
+def _mlp(n_in, hidden_sizes, n_out, tail=None, layer_norm=False, dropout=0.0):
+  """Linear/ReLU stack whose Linear layers sit at even Sequential indices (0, 2, 4, ...).  With `dropout` and / or
+  `layer_norm` a hidden layer is Linear, Dropout, LayerNorm, ReLU."""
   layers, width = [], n_in
   for h in hidden_sizes:
-    layers += [SkinnyLinear(width, h), nn.ReLU()]
+    layers.append(SkinnyLinear(width, h))
+    if dropout:
+      layers.append(Dropout(dropout))
+    if layer_norm:
+      layers.append(LayerNorm(h))
+    layers.append(nn.ReLU())
     width = h
   layers.append(SkinnyLinear(width, n_out))
   if tail is not None:
@@ -245,14 +301,15 @@ def _last_linear(seq):
 
 
 class QNet(nn.Module):
-  """obs -> Q(s, .): in -> 128 -> 128 -> out (models.py:6-24)."""
+  """obs -> Q(s, .): in -> 128 -> 128 -> out (models.py:6-24); `layer_norm` / `dropout` regularise the hidden layers
+  (extension: the reference has neither)."""
 
-  def __init__(self, input_size, output_size, hidden=128):
+  def __init__(self, input_size, output_size, hidden=128, layer_norm=False, dropout=0.0):
     super().__init__()
     self._input_size, self._output_size = input_size, output_size
     self._hidden_sizes = _as_sizes(hidden, 2)
     self._hidden_size = self._hidden_sizes[0]
-    self.net = _mlp(input_size, self._hidden_sizes, output_size)
+    self.net = _mlp(input_size, self._hidden_sizes, output_size, layer_norm=layer_norm, dropout=dropout)
 
   def forward(self, obs):
     return self.net(obs)
@@ -275,13 +332,14 @@ class DDPGActorNet(nn.Module):
 
 
 class DDPGCriticNet(nn.Module):
-  """(obs, action) -> Q; last layer U(-3e-3, 3e-3) (models.py:56-81)."""
+  """(obs, action) -> Q; last layer U(-3e-3, 3e-3) (models.py:56-81); `layer_norm` / `dropout` regularise the hidden
+  layers (extension)."""
 
-  def __init__(self, state_size, action_size, hidden_size):
+  def __init__(self, state_size, action_size, hidden_size, layer_norm=False, dropout=0.0):
     super().__init__()
     self.state_size, self.action_size, self.hidden_size = state_size, action_size, hidden_size
     self._weight_init = 3e-3
-    self.net = _mlp(state_size + action_size, _as_sizes(hidden_size, 2), 1)
+    self.net = _mlp(state_size + action_size, _as_sizes(hidden_size, 2), 1, layer_norm=layer_norm, dropout=dropout)
     out = _last_linear(self.net)
     nn.init.uniform_(out.weight, -self._weight_init, self._weight_init)
     nn.init.uniform_(out.bias, -self._weight_init, self._weight_init)
@@ -341,3 +399,55 @@ class ActorCriticNet(nn.Module):
     if isinstance(module, nn.Linear):
       nn.init.normal_(module.weight, mean=0., std=0.1)
       nn.init.constant_(module.bias, 0.1)
+
+
+class MemoryBlock(nn.Module):
+  """A residual layer with a memory over time, for policy and value networks on rollouts (extension; the reference's
+  networks see one observation at a time):
+
+      y = x + dropout(out(decay_attention(qkv(layer_norm(x)))))
+
+  `forward` takes a whole rollout [T, N, width] with gradients; `step` one env step [N, width] while acting: the same
+  function, the memory carried in `state` [N, heads, head_size, head_size] (csrc/trl_decay.hip).  start: where an episode
+  begins (the done column one step later; in `step`, the done flags of the step before).  decay: one constant per head, by
+  default 1 - 2^-j with j evenly from 3 to 10: memories of about 8 to 1,000 steps.  On the device only."""
+
+  def __init__(self, width, heads=4, head_size=32, dropout=0.0, decay=None):
+    super().__init__()
+    self.width, self.heads, self.head_size = int(width), int(heads), int(head_size)
+    if decay is None:
+      decay = 1.0 - torch.exp2(-torch.linspace(3.0, 10.0, self.heads))
+    decay = torch.as_tensor(decay, dtype=torch.float32).detach().clone()
+    if decay.shape != (self.heads,) or not bool(((decay >= 0) & (decay <= 1)).all()):
+      raise ValueError('MemoryBlock: decay must be %d values in [0, 1]' % self.heads)
+    self.norm = LayerNorm(self.width)
+    self.qkv = nn.Linear(self.width, 3 * self.heads * self.head_size)
+    self.out = nn.Linear(self.heads * self.head_size, self.width)
+    self.drop = Dropout(dropout)
+    self.register_buffer('decay', decay)
+
+  def _apply(self, fn, recurse=True):
+    """Casts of the module leave the decays in float32 (1 - 2^-10 is 1 in bfloat16)."""
+    decay = self.decay
+    super()._apply(fn, recurse)
+    self.decay = decay.to(self.decay.device)
+    return self
+
+  def _heads(self, x):
+    return self.qkv(self.norm(x)).unflatten(-1, (3, self.heads, self.head_size)).unbind(-3)
+
+  def initial_state(self, n):
+    return torch.zeros((n, self.heads, self.head_size, self.head_size), dtype=torch.float32, device=self.decay.device)
+
+  def forward(self, x, start=None, lengths=None, state=None):
+    """x [T, N, width] -> (y [T, N, width], the state behind each env's last step)."""
+    q, k, v = self._heads(x)
+    o, state = _F.decay_attention(q, k, v, self.decay, start=start, lengths=lengths, state=state)
+    return self.drop(self.out(o.flatten(-2)), residual=x), state
+
+  def step(self, x, state, start=None, out_state=None):
+    """x [N, width], state -> (y [N, width], the new state), without gradients; out_state may be `state`."""
+    with torch.no_grad():
+      q, k, v = self._heads(x)
+      o, state = _F.decay_attention_step(q, k, v, self.decay, state, start=start, out_state=out_state)
+      return self.drop(self.out(o.flatten(-2)), residual=x), state

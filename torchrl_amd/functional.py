@@ -5,6 +5,8 @@ There is no CPU implementation behind any of them: a CPU tensor raises TrlError.
 The loss functions are autograd Functions whose forward runs the fused kernel (loss AND
 its backward seeds in one pass) and whose backward only scales the saved seeds.
 """
+import ctypes as C
+
 import torch
 
 from . import _lib
@@ -565,6 +567,318 @@ def linear_u8(x, weight, bias, relu=False):
   Q-network on frames the replay ring keeps uint8 (the cast is exact: same values as the reference's
   float32 frames)."""
   return _LinearU8.apply(x, weight, bias, 1 if relu else 0)
+
+
+# ------------------------------------------------------------------------------ layer norm, dropout
+_LAYER_DTYPES = {torch.float32: _lib.TRL_F32, torch.bfloat16: _lib.TRL_BF16, torch.float16: _lib.TRL_F16}
+
+
+def _layer_dtype(t, what):
+  """C element type of a device tensor of the layer kernels (float32, bfloat16, float16)."""
+  _lib.require_device(t, what)
+  code = _LAYER_DTYPES.get(t.dtype)
+  if code is None:
+    raise TypeError('%s must be float32, bfloat16 or float16, got %s' % (what, t.dtype))
+  return code
+
+
+def _beside(t, other, what):
+  _lib.require_device(t, what)
+  if t.device != other.device:
+    raise ValueError('%s is on %s, the input on %s' % (what, t.device, other.device))
+  return t
+
+
+class _LayerNorm(torch.autograd.Function):
+  @staticmethod
+  def forward(ctx, x, weight, bias, eps, act):
+    code = _LAYER_DTYPES[x.dtype]
+    x = x.contiguous()
+    width = x.shape[-1]
+    rows = x.numel() // width
+    y = torch.empty_like(x)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad) else None
+    with torch.cuda.device(x.device):
+      _lib.check(_lib.lib().trl_layer_norm_fwd(
+          x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), rows, width, code, eps, act, y.data_ptr(),
+          stats.data_ptr() if stats is not None else None, stats.data_ptr() + 4 * rows if stats is not None else None,
+          _lib.stream_ptr(x.device)))
+    ctx.code, ctx.act, ctx.rows, ctx.width = code, act, rows, width
+    ctx.save_for_backward(x, weight, bias, stats)
+    return y
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, gy):
+    x, weight, bias, stats = ctx.saved_tensors
+    rows, width, lib = ctx.rows, ctx.width, _lib.lib()
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    gy = gy.contiguous()
+    dx = torch.empty_like(x) if need_x else None
+    dw = torch.empty_like(weight) if need_w else None
+    db = torch.empty_like(bias) if need_b else None
+    ws = None
+    if need_w or need_b:      # (a buffer of this call alone: two streams or two captured graphs never share one)
+      ws = torch.empty(lib.trl_layer_norm_bwd_workspace_bytes(rows, width, ctx.code), dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+      _lib.check(lib.trl_layer_norm_bwd(gy.data_ptr(), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), stats.data_ptr(),
+                                        stats.data_ptr() + 4 * rows, rows, width, ctx.code, ctx.act, _lib.ptr(dx),
+                                        _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), _lib.stream_ptr(x.device)))
+    return dx, dw, db, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False):
+  """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension (then ReLU), torch.nn.functional.layer_norm's
+  definition; one HIP launch forward, two backward (csrc/trl_norm.hip).
+
+  x: float32, bfloat16 or float16 on the device, any leading shape; weight, bias: [width] or None.  Statistics and
+  the parameters' gradients are float32 sums in a fixed order, each output is rounded to its type once."""
+  _layer_dtype(x, 'layer_norm: x')
+  if x.dim() < 1 or x.shape[-1] < 1:
+    raise ValueError('layer_norm: x needs a last dimension of at least 1, got %s' % (tuple(x.shape),))
+  eps = float(eps)
+  if not 1.2e-38 <= eps < 1e30:
+    raise ValueError('layer_norm: eps must be a positive float32, got %r' % eps)
+  params = []
+  for t, what in ((weight, 'weight'), (bias, 'bias')):
+    if t is not None:
+      _beside(t, x, 'layer_norm: ' + what)
+      if t.dim() != 1 or t.shape[0] != x.shape[-1]:
+        raise ValueError('layer_norm: %s must be [%d], got %s' % (what, x.shape[-1], tuple(t.shape)))
+      _layer_dtype(t, 'layer_norm: ' + what)
+      if t.dtype != torch.float32 or not t.is_contiguous():
+        t = t.float().contiguous()
+    params.append(t)
+  return _LayerNorm.apply(x, params[0], params[1], eps, 1 if relu else 0)
+
+
+def _dropout_launch(x, residual, code, p, seed, call, call_d):
+  y = torch.empty_like(x)
+  with torch.cuda.device(x.device):
+    _lib.check(_lib.lib().trl_dropout(x.data_ptr(), _lib.ptr(residual), x.numel(), code, p, seed, call, _lib.ptr(call_d),
+                                      y.data_ptr(), _lib.stream_ptr(x.device)))
+  return y
+
+
+class _Dropout(torch.autograd.Function):
+  @staticmethod
+  def forward(ctx, x, residual, p, seed, call, call_d):
+    code = _LAYER_DTYPES[x.dtype]
+    ctx.args = code, p, seed, call
+    ctx.save_for_backward(call_d)      # (written to since: autograd refuses the backward pass)
+    return _dropout_launch(x.contiguous(), residual.contiguous() if residual is not None else None, code, p, seed, call,
+                           call_d)
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, gy):
+    code, p, seed, call = ctx.args
+    call_d, = ctx.saved_tensors
+    gx = _dropout_launch(gy.contiguous(), None, code, p, seed, call, call_d) if ctx.needs_input_grad[0] else None
+    return gx, gy if ctx.needs_input_grad[1] else None, None, None, None, None
+
+
+def dropout(x, p, seed, call, residual=None):
+  """x with every element dropped with probability p and the others scaled by 1 / (1 - p), plus `residual`; one HIP
+  launch each way, no stored mask (csrc/trl_norm.hip).
+
+  Element i (in x's row-major order) of call number `call` is kept when word i % 4 of Philox-4x32-10 under key
+  `seed` and counter (call, i // 4) is at least p * 2^32: the mask is a function of (seed, call, i) alone and the
+  backward pass makes it again.  A dropped element gives 0 whatever it held.  call: a number, or a device int64 tensor of
+  one element (next_call) that is read when the kernel runs -- what a captured graph needs to draw a new mask at
+  every replay.  Every use within one call number gets the same mask: number the calls, or seed the layers, apart.
+  x, residual: float32, bfloat16 or float16, equal shapes and types; 0 <= p < 1."""
+  _layer_dtype(x, 'dropout: x')
+  p = float(p)
+  if not 0.0 <= p < 1.0:
+    raise ValueError('dropout: p must be in [0, 1), got %r' % p)
+  call_d = None
+  if torch.is_tensor(call):
+    _beside(call, x, 'dropout: call')
+    if call.dtype != torch.int64 or call.numel() != 1:
+      raise ValueError('dropout: call must be a number or an int64 tensor of one element')
+    call_d, call = call, 0
+  elif call < 0 or call >= 2 ** 64:
+    raise ValueError('dropout: call must be in [0, 2^64), got %r' % call)
+  if residual is not None:
+    _beside(residual, x, 'dropout: residual')
+    if residual.shape != x.shape or residual.dtype != x.dtype:
+      raise ValueError('dropout: residual must be %s %s like x, got %s %s' %
+                       (tuple(x.shape), x.dtype, tuple(residual.shape), residual.dtype))
+  return _Dropout.apply(x, residual, p, int(seed) & (2 ** 64 - 1), int(call), call_d)
+
+
+def next_call(counter):
+  """A fresh device tensor holding the value of `counter` (int64, one element, on the device), which goes up by one: the
+  call number of one dropout call, drawn on the stream -- so also at every replay of a captured graph."""
+  _lib.require_device(counter, 'next_call: counter')
+  if counter.dtype != torch.int64 or counter.numel() != 1:
+    raise ValueError('next_call: counter must be an int64 tensor of one element')
+  call = torch.empty(1, dtype=torch.int64, device=counter.device)
+  with torch.cuda.device(counter.device):
+    _lib.check(_lib.lib().trl_next_call(counter.data_ptr(), call.data_ptr(), _lib.stream_ptr(counter.device)))
+  return call
+
+
+# ------------------------------------------------------------------------------ decay attention
+_MAX_HEAD = 128
+
+
+def _decay_operands(fn, q, k, v, decay, lead):
+  """Checks what the sequence and the single-step form share; lead: dimensions in front of [H, D]."""
+  code = _layer_dtype(q, fn + ': q')
+  for t, what in ((k, 'k'), (v, 'v')):
+    _beside(t, q, '%s: %s' % (fn, what))
+    if t.dtype != q.dtype:
+      raise TypeError('%s: %s is %s, q is %s' % (fn, what, t.dtype, q.dtype))
+  if q.dim() != lead + 2 or k.shape != q.shape or v.dim() != lead + 2 or v.shape[:-1] != q.shape[:-1]:
+    raise ValueError('%s: expected q, k [%sN, H, Dk] and v [%sN, H, Dv], got %s %s %s' %
+                     ((fn,) + ('T, ' if lead == 2 else '',) * 2 + (tuple(q.shape), tuple(k.shape), tuple(v.shape))))
+  H, dk, dv = q.shape[-2], q.shape[-1], v.shape[-1]
+  if H < 1 or not 1 <= dk <= _MAX_HEAD or not 1 <= dv <= _MAX_HEAD:
+    raise ValueError('%s: needs at least one head and head sizes in [1, %d], got H=%d Dk=%d Dv=%d' %
+                     (fn, _MAX_HEAD, H, dk, dv))
+  _beside(decay, q, fn + ': decay')
+  if decay.dtype != torch.float32 or decay.dim() != 1 or decay.shape[0] != H:
+    raise ValueError('%s: decay must be float32 [%d], got %s %s' % (fn, H, decay.dtype, tuple(decay.shape)))
+  if decay.requires_grad:
+    raise ValueError('%s: decay is a constant of the layer and gets no gradient' % fn)
+  return code
+
+
+def _start_flags(fn, start, q, shape):
+  if start is None:
+    return None, 0
+  _beside(start, q, fn + ': start')
+  if tuple(start.shape) != shape:
+    raise ValueError('%s: start must be %s, got %s' % (fn, shape, tuple(start.shape)))
+  if start.dtype not in (torch.float32, torch.bool, torch.uint8):
+    raise TypeError('%s: start must be float32, bool or uint8, got %s' % (fn, start.dtype))
+  return start.contiguous(), _lib.TRL_F32 if start.dtype == torch.float32 else _lib.TRL_U8
+
+
+def _state_like(fn, state, q, shape, what='state'):
+  _beside(state, q, '%s: %s' % (fn, what))
+  if state.dtype != torch.float32 or tuple(state.shape) != shape:
+    raise ValueError('%s: %s must be float32 %s, got %s %s' % (fn, what, shape, state.dtype, tuple(state.shape)))
+
+
+def _dense_heads(t):
+  return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _scan_strides(q, k, v):
+  return (C.c_int64 * 9)(*(q.stride()[:3] + k.stride()[:3] + v.stride()[:3]))
+
+
+class _DecayAttention(torch.autograd.Function):
+  @staticmethod
+  def forward(ctx, q, k, v, state, decay, start, lengths, start_code, scale):
+    T, N, H, dk = q.shape
+    dv, code, lib = v.shape[3], _LAYER_DTYPES[q.dtype], _lib.lib()
+    out = torch.empty((T, N, H, dv), dtype=q.dtype, device=q.device)
+    last = torch.empty((N, H, dk, dv), dtype=torch.float32, device=q.device)
+    nbytes = lib.trl_decay_attention_workspace_bytes(T, N, H, dk, dv, 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
+    with torch.cuda.device(q.device):
+      _lib.check(lib.trl_decay_attention_fwd(
+          q.data_ptr(), k.data_ptr(), v.data_ptr(), _scan_strides(q, k, v), decay.data_ptr(), _lib.ptr(start), start_code,
+          _lib.ptr(lengths), _lib.ptr(state), T, N, H, dk, dv, code, scale, out.data_ptr(), last.data_ptr(), _lib.ptr(ws),
+          _lib.stream_ptr(q.device)))
+    ctx.set_materialize_grads(False)
+    ctx.args = start_code, scale
+    ctx.save_for_backward(q, k, v, state, decay, start, lengths)
+    return out, last
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, gy, glast):
+    q, k, v, state, decay, start, lengths = ctx.saved_tensors
+    start_code, scale = ctx.args
+    T, N, H, dk = q.shape
+    dv, code, lib = v.shape[3], _LAYER_DTYPES[q.dtype], _lib.lib()
+    gy = torch.zeros((T, N, H, dv), dtype=q.dtype, device=q.device) if gy is None else gy.contiguous()
+    glast = glast.contiguous() if glast is not None else None
+    gq = torch.empty((T, N, H, dk), dtype=q.dtype, device=q.device)
+    gk = torch.empty_like(gq)
+    gv = torch.empty_like(gy)
+    gs = torch.empty((N, H, dk, dv), dtype=torch.float32, device=q.device) if ctx.needs_input_grad[3] else None
+    nbytes = lib.trl_decay_attention_workspace_bytes(T, N, H, dk, dv, 1)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
+    with torch.cuda.device(q.device):
+      _lib.check(lib.trl_decay_attention_bwd(
+          gy.data_ptr(), _lib.ptr(glast), q.data_ptr(), k.data_ptr(), v.data_ptr(), _scan_strides(q, k, v), decay.data_ptr(),
+          _lib.ptr(start), start_code, _lib.ptr(lengths), _lib.ptr(state), T, N, H, dk, dv, code, scale, gq.data_ptr(),
+          gk.data_ptr(), gv.data_ptr(), _lib.ptr(gs), _lib.ptr(ws), _lib.stream_ptr(q.device)))
+    return gq, gk, gv, gs, None, None, None, None, None
+
+
+def decay_attention(q, k, v, decay, scale=None, start=None, lengths=None, state=None):
+  """Linear attention with a decay per head over a rollout [T, N, .] (csrc/trl_decay.hip): the sequence form of a memory
+  whose single-step form is decay_attention_step.  For every env and head, with S a [Dk, Dv] matrix,
+
+      S_t = (0 if start_t else decay * S_{t-1}) + k_t v_t^T,     out_t = scale * q_t^T S_t.
+
+  q, k: [T, N, H, Dk], v: [T, N, H, Dv], float32, bfloat16 or float16, head sizes up to 128; read through their strides
+  (slices of one projection, and heads shared by expand(), are not copied).  decay: float32 [H] in [0, 1], a constant.
+  scale: Dk ** -0.5 by default.  start: [T, N] float32, bool or uint8, not zero where an episode begins (the done column one
+  step later).  lengths: [N] int32 or int64; env n's steps from lengths[n] on are neither read nor counted, their outputs
+  and gradients are zero.  state: float32 [N, H, Dk, Dv] before the first step, None = zeros.
+
+  Returns (out [T, N, H, Dv], the state after each env's last step); both carry gradients to q, k, v and state."""
+  fn = 'decay_attention'
+  _decay_operands(fn, q, k, v, decay, 2)
+  T, N, H, dk = q.shape
+  start, start_code = _start_flags(fn, start, q, (T, N))
+  if lengths is not None:
+    _beside(lengths, q, fn + ': lengths')
+    if lengths.dtype not in (torch.int32, torch.int64) or tuple(lengths.shape) != (N,):
+      raise ValueError('%s: lengths must be int32 or int64 [%d], got %s %s' % (fn, N, lengths.dtype, tuple(lengths.shape)))
+    lengths = (lengths.clamp(0, T).to(torch.int32) if lengths.dtype == torch.int64 else lengths).contiguous()
+  if state is not None:
+    _state_like(fn, state, q, (N, H, dk, v.shape[3]))
+    state = state.contiguous()
+  scale = dk ** -0.5 if scale is None else float(scale)
+  return _DecayAttention.apply(_dense_heads(q), _dense_heads(k), _dense_heads(v), state, decay.contiguous(), start, lengths,
+                               start_code, scale)
+
+
+def decay_attention_step(q, k, v, decay, state, scale=None, start=None, out_state=None):
+  """One env step of decay_attention: q, k [N, H, Dk], v [N, H, Dv], state float32 [N, H, Dk, Dv], start [N] -> (out
+  [N, H, Dv], the new state), one launch.  out_state: where the new state goes (may be `state` itself), a new tensor
+  by default.  For acting: it carries no gradients and refuses inputs that ask for them."""
+  fn = 'decay_attention_step'
+  code = _decay_operands(fn, q, k, v, decay, 1)
+  N, H, dk = q.shape
+  dv = v.shape[2]
+  start, start_code = _start_flags(fn, start, q, (N,))
+  shape = (N, H, dk, dv)
+  _state_like(fn, state, q, shape)
+  if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+    raise ValueError('%s has no gradient: call it under torch.no_grad(), or decay_attention with T = 1' % fn)
+  given = state
+  state = state.contiguous()
+  if out_state is None:
+    out_state = torch.empty(shape, dtype=torch.float32, device=q.device)
+  else:
+    _state_like(fn, out_state, q, shape, 'out_state')
+    if not out_state.is_contiguous():
+      raise ValueError('%s: out_state must be contiguous' % fn)
+    if out_state.requires_grad and torch.is_grad_enabled():
+      raise ValueError('%s: out_state must not require a gradient' % fn)
+    apart = abs(out_state.data_ptr() - state.data_ptr())
+    if 0 < apart < 4 * state.numel():
+      raise ValueError('%s: out_state overlaps state without being it' % fn)
+    if state is not given and out_state.untyped_storage().data_ptr() == given.untyped_storage().data_ptr():
+      raise ValueError('%s: out_state shares memory with a state that is not contiguous' % fn)
+  out = torch.empty((N, H, dv), dtype=q.dtype, device=q.device)
+  scale = dk ** -0.5 if scale is None else float(scale)
+  q, k, v, decay = q.contiguous(), k.contiguous(), v.contiguous(), decay.contiguous()
+  with torch.cuda.device(q.device):
+    _lib.check(_lib.lib().trl_decay_attention_step(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), _lib.ptr(start), start_code, state.data_ptr(), N, H, dk,
+        dv, code, scale, out.data_ptr(), out_state.data_ptr(), _lib.stream_ptr(q.device)))
+  return out, out_state
 
 
 def _fill_desc(d, weights, biases):
