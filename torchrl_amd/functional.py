@@ -598,7 +598,7 @@ class _LayerNorm(torch.autograd.Function):
     rows = x.numel() // width
     y = torch.empty_like(x)
     stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad) else None
-    with torch.cuda.device(x.device):
+    with _lib.device_guard(x.device):
       _lib.check(_lib.lib().trl_layer_norm_fwd(
           x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), rows, width, code, eps, act, y.data_ptr(),
           stats.data_ptr() if stats is not None else None, stats.data_ptr() + 4 * rows if stats is not None else None,
@@ -620,7 +620,7 @@ class _LayerNorm(torch.autograd.Function):
     ws = None
     if need_w or need_b:      # (a buffer of this call alone: two streams or two captured graphs never share one)
       ws = torch.empty(lib.trl_layer_norm_bwd_workspace_bytes(rows, width, ctx.code), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
+    with _lib.device_guard(x.device):
       _lib.check(lib.trl_layer_norm_bwd(gy.data_ptr(), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), stats.data_ptr(),
                                         stats.data_ptr() + 4 * rows, rows, width, ctx.code, ctx.act, _lib.ptr(dx),
                                         _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), _lib.stream_ptr(x.device)))
@@ -654,7 +654,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False):
 
 def _dropout_launch(x, residual, code, p, seed, call, call_d):
   y = torch.empty_like(x)
-  with torch.cuda.device(x.device):
+  with _lib.device_guard(x.device):
     _lib.check(_lib.lib().trl_dropout(x.data_ptr(), _lib.ptr(residual), x.numel(), code, p, seed, call, _lib.ptr(call_d),
                                       y.data_ptr(), _lib.stream_ptr(x.device)))
   return y
@@ -715,7 +715,7 @@ def next_call(counter):
   if counter.dtype != torch.int64 or counter.numel() != 1:
     raise ValueError('next_call: counter must be an int64 tensor of one element')
   call = torch.empty(1, dtype=torch.int64, device=counter.device)
-  with torch.cuda.device(counter.device):
+  with _lib.device_guard(counter.device):
     _lib.check(_lib.lib().trl_next_call(counter.data_ptr(), call.data_ptr(), _lib.stream_ptr(counter.device)))
   return call
 
@@ -780,7 +780,7 @@ class _DecayAttention(torch.autograd.Function):
     last = torch.empty((N, H, dk, dv), dtype=torch.float32, device=q.device)
     nbytes = lib.trl_decay_attention_workspace_bytes(T, N, H, dk, dv, 0)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-    with torch.cuda.device(q.device):
+    with _lib.device_guard(q.device):
       _lib.check(lib.trl_decay_attention_fwd(
           q.data_ptr(), k.data_ptr(), v.data_ptr(), _scan_strides(q, k, v), decay.data_ptr(), _lib.ptr(start), start_code,
           _lib.ptr(lengths), _lib.ptr(state), T, N, H, dk, dv, code, scale, out.data_ptr(), last.data_ptr(), _lib.ptr(ws),
@@ -805,7 +805,7 @@ class _DecayAttention(torch.autograd.Function):
     gs = torch.empty((N, H, dk, dv), dtype=torch.float32, device=q.device) if ctx.needs_input_grad[3] else None
     nbytes = lib.trl_decay_attention_workspace_bytes(T, N, H, dk, dv, 1)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-    with torch.cuda.device(q.device):
+    with _lib.device_guard(q.device):
       _lib.check(lib.trl_decay_attention_bwd(
           gy.data_ptr(), _lib.ptr(glast), q.data_ptr(), k.data_ptr(), v.data_ptr(), _scan_strides(q, k, v), decay.data_ptr(),
           _lib.ptr(start), start_code, _lib.ptr(lengths), _lib.ptr(state), T, N, H, dk, dv, code, scale, gq.data_ptr(),
@@ -874,7 +874,7 @@ def decay_attention_step(q, k, v, decay, state, scale=None, start=None, out_stat
   out = torch.empty((N, H, dv), dtype=q.dtype, device=q.device)
   scale = dk ** -0.5 if scale is None else float(scale)
   q, k, v, decay = q.contiguous(), k.contiguous(), v.contiguous(), decay.contiguous()
-  with torch.cuda.device(q.device):
+  with _lib.device_guard(q.device):
     _lib.check(_lib.lib().trl_decay_attention_step(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), _lib.ptr(start), start_code, state.data_ptr(), N, H, dk,
         dv, code, scale, out.data_ptr(), out_state.data_ptr(), _lib.stream_ptr(q.device)))
