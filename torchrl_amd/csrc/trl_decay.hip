@@ -476,12 +476,21 @@ __global__ __launch_bounds__(kThreads) void k_join(float *__restrict__ seg_state
   float *p = seg_state + nh * segs * size + (e - nh * size);
   const float *coef = seg_coef + nh * segs;
   float cur = state_in ? state_in[e] : 0.f;
-  for (int i = 0; i < segs; ++i) {
-    const int sg = reverse ? segs - 1 - i : i;
-    const bool last = i == segs - 1;
-    const float u = last ? 0.f : p[sg * size], cf = last ? 0.f : coef[sg];
-    p[sg * size] = cur;
-    cur = cf < 0.f ? u : fmaf(cf, cur, u);
+  const int first = reverse ? segs - 1 : 0, dir = reverse ? -1 : 1;
+  for (int i0 = 0; i0 < segs; i0 += 8) {
+    float u[8], cf[8];         // eight contributions in flight
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool on = i0 + i < segs - 1;      // (the last one moves nothing on)
+      const int sg = first + dir * (i0 + i);
+      u[i] = on ? p[sg * size] : 0.f;
+      cf[i] = on ? coef[sg] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i0 + i < segs) p[(first + dir * (i0 + i)) * size] = cur;
+      cur = cf[i] < 0.f ? u[i] : fmaf(cf[i], cur, u[i]);
+    }
   }
 }
 

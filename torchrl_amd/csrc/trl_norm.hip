@@ -34,37 +34,59 @@ __device__ __forceinline__ float row_sum(float v, float *red) {
   }
 }
 
+// 16 B of a row as loaded, zero past the row's end; nothing touches it before its row's turn
 template <typename T>
-__device__ __forceinline__ void load_slot(const T *row, int64_t width, int64_t c, float fill, float (&f)[TrlIo<T>::V]) {
+struct Slot {
+  T t[TrlIo<T>::V];
+};
+
+// VEC: a row is whole slots, so that one comparison a slot decides
+template <bool VEC, typename T>
+__device__ __forceinline__ void load_slot(Slot<T> &q, const T *row, int64_t width, int64_t c) {
   constexpr int V = TrlIo<T>::V;
   if (c + V <= width) {
-    trl_load16(row + c, f);
+    __builtin_memcpy(q.t, row + c, 16);
+  } else if constexpr (VEC) {
+    q = Slot<T>{};
   } else {
-    const int64_t left = width - c;
-    trl_load_part(row + c, left > 0 ? (int)left : 0, fill, f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      q.t[i] = (T)0.f;
+      if (c + i < width) q.t[i] = row[c + i];
+    }
   }
 }
 
 template <typename T>
+__device__ __forceinline__ void slot_value(const Slot<T> &q, float (&f)[TrlIo<T>::V]) {
+#pragma unroll
+  for (int i = 0; i < TrlIo<T>::V; ++i) f[i] = (float)q.t[i];
+}
+
+template <bool VEC, typename T>
 __device__ __forceinline__ void store_slot(T *row, int64_t width, int64_t c, const float (&f)[TrlIo<T>::V]) {
   constexpr int V = TrlIo<T>::V;
   if (c + V <= width)
     trl_store16(row + c, f);
-  else if (c < width)
+  else if (!VEC && c < width)
     trl_store_part(row + c, (int)(width - c), f);
 }
 
 // V parameters (float32) of the columns from c on
-template <int V>
+template <int V, bool VEC>
 __device__ __forceinline__ void load_param(const float *p, int64_t width, int64_t c, float none, float (&f)[V]) {
+  if (p != nullptr && c + V <= width) {
+    __builtin_memcpy(f, p + c, 4 * V);
+  } else {
 #pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = (p != nullptr && c + i < width) ? p[c + i] : none;
+    for (int i = 0; i < V; ++i) f[i] = (!VEC && p != nullptr && c + i < width) ? p[c + i] : none;
+  }
 }
 
 __device__ __forceinline__ float relu_keep_nan(float z) { return z < 0.f ? 0.f : z; }
 __device__ __forceinline__ float clip(float z, float g) { return z <= 0.f ? 0.f : g; }
 
-template <typename T, int LPR, int NV, bool ACT>
+template <typename T, int LPR, int NV, bool ACT, bool VEC>
 __global__ __launch_bounds__(kThreads) void k_norm_fwd(const T *__restrict__ x, const float *__restrict__ w,
                                                        const float *__restrict__ b, int64_t rows, int64_t width, float eps,
                                                        T *__restrict__ y, float *__restrict__ mean,
@@ -73,21 +95,32 @@ __global__ __launch_bounds__(kThreads) void k_norm_fwd(const T *__restrict__ x, 
   __shared__ float red[4];
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const float inv = 1.0f / (float)width;
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + group;
+  Slot<T> next[NV];
+  if (row < rows) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) load_slot<VEC>(next[j], x + row * width, width, (int64_t)(j * LPR + lane) * V);
+  }
   float wv[NV][V], bv[NV][V];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    load_param<V>(w, width, (int64_t)(j * LPR + lane) * V, 1.f, wv[j]);
-    load_param<V>(b, width, (int64_t)(j * LPR + lane) * V, 0.f, bv[j]);
+    load_param<V, VEC>(w, width, (int64_t)(j * LPR + lane) * V, 1.f, wv[j]);
+    load_param<V, VEC>(b, width, (int64_t)(j * LPR + lane) * V, 0.f, bv[j]);
   }
-  for (int64_t row = (int64_t)blockIdx.x * RPB + group; row < rows; row += (int64_t)gridDim.x * RPB) {
-    const T *xr = x + row * width;
+  for (; row < rows; row += step) {
     float v[NV][V];
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      load_slot(xr, width, (int64_t)(j * LPR + lane) * V, 0.f, v[j]);
+      slot_value(next[j], v[j]);
 #pragma unroll
       for (int i = 0; i < V; ++i) s += v[j][i];
+    }
+    // the next row is on its way while this one is worked on
+    if (row + step < rows) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) load_slot<VEC>(next[j], x + (row + step) * width, width, (int64_t)(j * LPR + lane) * V);
     }
     const float m = row_sum<LPR>(s, red) * inv;
     float q = 0.f;
@@ -95,7 +128,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_fwd(const T *__restrict__ x, 
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float d = (int64_t)(j * LPR + lane) * V + i < width ? v[j][i] - m : 0.f;
+        const float d = (int64_t)(j * LPR + lane) * V + (VEC ? 0 : i) < width ? v[j][i] - m : 0.f;
         v[j][i] = d;
         q = fmaf(d, d, q);
       }
@@ -111,12 +144,12 @@ __global__ __launch_bounds__(kThreads) void k_norm_fwd(const T *__restrict__ x, 
         const float z = fmaf(v[j][i] * r, wv[j][i], bv[j][i]);
         v[j][i] = ACT ? relu_keep_nan(z) : z;
       }
-      store_slot(y + row * width, width, (int64_t)(j * LPR + lane) * V, v[j]);
+      store_slot<VEC>(y + row * width, width, (int64_t)(j * LPR + lane) * V, v[j]);
     }
   }
 }
 
-template <typename T, int LPR, int NV, bool ACT>
+template <typename T, int LPR, int NV, bool ACT, bool VEC>
 __global__ __launch_bounds__(kThreads) void k_norm_bwd(const T *__restrict__ gy, const T *__restrict__ x,
                                                        const float *__restrict__ w, const float *__restrict__ b,
                                                        const float *__restrict__ mean, const float *__restrict__ rstd,
@@ -127,28 +160,43 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd(const T *__restrict__ gy,
   __shared__ float fold[kThreads * V];
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   const float inv = 1.0f / (float)width;
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + group;
+  Slot<T> next_x[NV], next_g[NV];
+  float m_next = 0.f, r_next = 0.f;
+  auto bring = [&](int64_t at) {
+    m_next = mean[at], r_next = rstd[at];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int64_t col = (int64_t)(j * LPR + lane) * V;
+      load_slot<VEC>(next_x[j], x + at * width, width, col);
+      load_slot<VEC>(next_g[j], gy + at * width, width, col);
+    }
+  };
+  if (row < rows) bring(row);
   float wv[NV][V], bv[NV][V], dw[NV][V], db[NV][V];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    load_param<V>(w, width, (int64_t)(j * LPR + lane) * V, 1.f, wv[j]);
-    load_param<V>(b, width, (int64_t)(j * LPR + lane) * V, 0.f, bv[j]);
+    load_param<V, VEC>(w, width, (int64_t)(j * LPR + lane) * V, 1.f, wv[j]);
+    if (ACT) load_param<V, VEC>(b, width, (int64_t)(j * LPR + lane) * V, 0.f, bv[j]);
 #pragma unroll
     for (int i = 0; i < V; ++i) dw[j][i] = db[j][i] = 0.f;
   }
-  for (int64_t row = (int64_t)blockIdx.x * RPB + group; row < rows; row += (int64_t)gridDim.x * RPB) {
-    const float m = mean[row], r = rstd[row];
+  for (; row < rows; row += step) {
+    const float m = m_next, r = r_next;
     float n[NV][V], g[NV][V];
     float a = 0.f, c = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int64_t col = (int64_t)(j * LPR + lane) * V;
-      load_slot(x + row * width, width, col, m, n[j]);      // (past the row's end: n = 0)
-      load_slot(gy + row * width, width, col, 0.f, g[j]);
+      slot_value(next_x[j], n[j]);
+      slot_value(next_g[j], g[j]);
     }
+    if (row + step < rows) bring(row + step);      // the next row is on its way while this one is worked on
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
+        // (past the row's end g is 0, and so is every product with u)
         const float u = (n[j][i] - m) * r;
         // the forward's own expression: its y > 0 decides, to the bit
         const float t = ACT ? clip(fmaf(u, wv[j][i], bv[j][i]), g[j][i]) : g[j][i];
@@ -166,7 +214,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd(const T *__restrict__ gy,
       for (int j = 0; j < NV; ++j) {
 #pragma unroll
         for (int i = 0; i < V; ++i) g[j][i] = r * (g[j][i] - fmaf(n[j][i], cm, am));
-        store_slot(dx + row * width, width, (int64_t)(j * LPR + lane) * V, g[j]);
+        store_slot<VEC>(dx + row * width, width, (int64_t)(j * LPR + lane) * V, g[j]);
       }
     }
   }
@@ -276,21 +324,34 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_wide_dw(const T *__restri
   out[width + c] = db;
 }
 
-// dw, db = the parts added in order: 16 columns a workgroup, 16 strips of parts added by a tree of fixed shape
-__global__ __launch_bounds__(kThreads) void k_norm_fold(const float *__restrict__ part, int parts, int64_t width,
-                                                        float *__restrict__ dw, float *__restrict__ db) {
-  __shared__ float sm[16][17];
+// dw, db = the parts added in a fixed order: 16 columns a workgroup, 64 strips of parts, eight loads of a strip in flight
+__global__ __launch_bounds__(1024) void k_norm_fold(const float *__restrict__ part, int parts, int64_t width,
+                                                    float *__restrict__ dw, float *__restrict__ db) {
+  __shared__ float sm[64][17], top[4][16];
   const int lc = threadIdx.x & 15, strip = threadIdx.x >> 4;
   const int64_t c = (int64_t)blockIdx.x * 16 + lc, total = 2 * width;
   float s = 0.f;
-  if (c < total)
-    for (int p = strip; p < parts; p += 16) s += part[(int64_t)p * total + c];
+  if (c < total) {
+    for (int p0 = strip; p0 < parts; p0 += 64 * 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = p0 + 64 * i < parts ? part[(int64_t)(p0 + 64 * i) * total + c] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[i];
+    }
+  }
   sm[strip][lc] = s;
   __syncthreads();
-  if (strip == 0 && c < total) {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t += sm[i][lc];
+  if (threadIdx.x < 256) {
+    // strips 4 k .. 4 k + 3, then the 16 sums of them
+    float t = (sm[4 * strip][lc] + sm[4 * strip + 1][lc]) + (sm[4 * strip + 2][lc] + sm[4 * strip + 3][lc]);
+    t += __shfl_xor(t, 16, 64);
+    t += __shfl_xor(t, 32, 64);
+    if ((threadIdx.x & 63) < 16) top[threadIdx.x >> 6][lc] = t;
+  }
+  __syncthreads();
+  if (threadIdx.x < 16 && c < total) {
+    const float t = (top[0][lc] + top[1][lc]) + (top[2][lc] + top[3][lc]);
     if (c < width) {
       if (dw != nullptr) dw[c] = t;
     } else if (db != nullptr) {
@@ -318,10 +379,10 @@ Shape shape_of(int64_t width, int v) {
   return {0, 0};
 }
 
-#define FOR_ACT(act, ...)                                    \
+#define FOR_BOOL(value, NAME, ...)                           \
   do {                                                       \
-    if (act) { constexpr bool ACT = true; __VA_ARGS__; }     \
-    else { constexpr bool ACT = false; __VA_ARGS__; }        \
+    if (value) { constexpr bool NAME = true; __VA_ARGS__; }  \
+    else { constexpr bool NAME = false; __VA_ARGS__; }       \
   } while (0)
 
 #define NORM_SHAPES(sh, ...)                                              \
@@ -370,12 +431,14 @@ extern "C" int trl_layer_norm_fwd(const void *x, const float *weight, const floa
   TRL_FOR_DTYPE(dtype, {
     if (sh.lpr == 0) {
       const int grid = (int)std::min<int64_t>(rows, 2048);
-      FOR_ACT(act, (k_norm_fwd_wide<T, ACT><<<grid, kThreads, 0, st>>>((const T *)x, weight, bias, rows, width, (float)eps,
+      FOR_BOOL(act, ACT, (k_norm_fwd_wide<T, ACT><<<grid, kThreads, 0, st>>>((const T *)x, weight, bias, rows, width, (float)eps,
                                                                        (T *)y, mean, rstd)));
     } else {
       const int grid = (int)std::min<int64_t>(trl_cdiv(rows, kThreads / sh.lpr), 2048);
-      NORM_SHAPES(sh, FOR_ACT(act, (k_norm_fwd<T, LPR, NV, ACT><<<grid, kThreads, 0, st>>>(
-                                       (const T *)x, weight, bias, rows, width, (float)eps, (T *)y, mean, rstd))));
+      const bool vec = width % TrlIo<T>::V == 0;
+      NORM_SHAPES(sh, FOR_BOOL(vec, VEC, FOR_BOOL(act, ACT, (k_norm_fwd<T, LPR, NV, ACT, VEC><<<grid, kThreads, 0, st>>>(
+                                                                (const T *)x, weight, bias, rows, width, (float)eps, (T *)y,
+                                                                mean, rstd)))));
     }
   });
   TRL_CHECK_LAUNCH(fn);
@@ -404,19 +467,21 @@ extern "C" int trl_layer_norm_bwd(const void *gy, const void *x, const float *we
     if (sh.lpr == 0) {
       const int grid = (int)std::min<int64_t>(rows, 2048);
       if (dx != nullptr && rows > 0)
-        FOR_ACT(act, (k_norm_bwd_wide_dx<T, ACT><<<grid, kThreads, 0, st>>>((const T *)gy, (const T *)x, weight, bias, mean,
+        FOR_BOOL(act, ACT, (k_norm_bwd_wide_dx<T, ACT><<<grid, kThreads, 0, st>>>((const T *)gy, (const T *)x, weight, bias, mean,
                                                                             rstd, rows, width, (T *)dx)));
       if (params)
-        FOR_ACT(act, (k_norm_bwd_wide_dw<T, ACT><<<dim3((int)trl_cdiv(width, kThreads), parts), kThreads, 0, st>>>(
+        FOR_BOOL(act, ACT, (k_norm_bwd_wide_dw<T, ACT><<<dim3((int)trl_cdiv(width, kThreads), parts), kThreads, 0, st>>>(
                          (const T *)gy, (const T *)x, weight, bias, mean, rstd, rows, width, part)));
     } else {
-      NORM_SHAPES(sh, FOR_ACT(act, (k_norm_bwd<T, LPR, NV, ACT><<<parts, kThreads, 0, st>>>(
-                                       (const T *)gy, (const T *)x, weight, bias, mean, rstd, rows, width, (T *)dx, part))));
+      const bool vec = width % TrlIo<T>::V == 0;
+      NORM_SHAPES(sh, FOR_BOOL(vec, VEC, FOR_BOOL(act, ACT, (k_norm_bwd<T, LPR, NV, ACT, VEC><<<parts, kThreads, 0, st>>>(
+                                                                (const T *)gy, (const T *)x, weight, bias, mean, rstd, rows,
+                                                                width, (T *)dx, part)))));
     }
   });
   TRL_CHECK_LAUNCH(fn);
   if (params) {
-    k_norm_fold<<<(int)trl_cdiv(2 * width, 16), kThreads, 0, st>>>(part, parts, width, dweight, dbias);
+    k_norm_fold<<<(int)trl_cdiv(2 * width, 16), 1024, 0, st>>>(part, parts, width, dweight, dbias);
     TRL_CHECK_LAUNCH(fn);
   }
   return TRL_OK;
@@ -430,11 +495,11 @@ extern "C" int trl_layer_norm_bwd(const void *gy, const void *x, const float *we
 // Bound by memory in float32; the generator costs 20 32 x 32 -> 64 bit products for four elements.
 namespace {
 
-__device__ __forceinline__ void philox4(uint64_t seed, uint64_t call, uint64_t group, uint32_t (&c)[4]) {
+__device__ __forceinline__ void philox4(uint64_t seed, uint64_t call, uint32_t group, uint32_t group_hi, uint32_t (&c)[4]) {
   c[0] = (uint32_t)call;
   c[1] = (uint32_t)(call >> 32);
-  c[2] = (uint32_t)group;
-  c[3] = (uint32_t)(group >> 32) | 0x80000000u;
+  c[2] = group;
+  c[3] = group_hi | 0x80000000u;
   uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
@@ -451,7 +516,12 @@ __global__ __launch_bounds__(kThreads) void k_dropout(const T *__restrict__ x, c
   constexpr int V = TrlIo<T>::V;
   if (call_d != nullptr) call = (uint64_t)call_d[0];
   const int64_t slots = (n + V - 1) / V;
-  for (int64_t s = (int64_t)blockIdx.x * kThreads + threadIdx.x; s < slots; s += (int64_t)gridDim.x * kThreads) {
+  for (int64_t s0 = (int64_t)blockIdx.x * kThreads; s0 < slots; s0 += (int64_t)gridDim.x * kThreads) {
+    const int64_t s = s0 + threadIdx.x;
+    if (s >= slots) return;
+    // a workgroup's slots begin at a multiple of 256: one high word for all of them, and two of the generator's products
+    // are the same for the whole wave
+    const uint32_t group_hi = (uint32_t)((uint64_t)s0 * (V / 4) >> 32);
     const int64_t i = s * V;
     const bool whole = i + V <= n;
     float v[V], e[V];
@@ -465,7 +535,7 @@ __global__ __launch_bounds__(kThreads) void k_dropout(const T *__restrict__ x, c
 #pragma unroll
     for (int g = 0; g < V / 4; ++g) {
       uint32_t u[4];
-      philox4(seed, call, (uint64_t)(s * (V / 4) + g), u);
+      philox4(seed, call, (uint32_t)((uint64_t)s * (V / 4) + g), group_hi, u);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float d = u[k] >= threshold ? v[4 * g + k] * scale : 0.f;      // (whatever a dropped element holds)
