@@ -25,57 +25,15 @@
 // Values that are not finite stay where the recurrence puts them: masks are selections, never products with zero -- except
 // of b's and c's steps inside a chunk, so a chunk whose b or c holds an infinity or a NaN is taken one step at a time.
 #include <algorithm>
-#include <type_traits>
 
-#include "trl_io.h"
+#include "trl_decay_scan.h"
+
+using namespace trl_decay;
 
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
 constexpr int kThreads = 256;
 constexpr int kMaxDim = 128;
-
-struct Operand {
-  const void *p;
-  int64_t st, sn, sh;      // strides of time, env and head, in elements; the head's own dimension is dense
-};
-
-struct Scan {
-  Operand a, b, c;
-  void *out;               // [T, N, H, dc] dense
-  const float *decay;
-  const void *start;       // [T, N] or null
-  const int32_t *lengths;  // [N] or null
-  const float *state_in;   // [N, H, ...] or null; transposed: [.., dc, da]
-  float *state_out;        // [N, H, da, dc] or null
-  float *seg_state;        // [N, H, segs, .., ..] or null (one segment)
-  float *seg_coef;         // [N, H, segs]
-  int64_t T, N;
-  int32_t H, da, dc, segs, seg_len;
-  int32_t start_u8, reverse, state_t;
-  float s_inter, s_intra, s_state;
-};
-
-// lambda^n in double, n < 32: each power is rounded to f32 once
-__device__ __forceinline__ double power(double lam, int n) {
-  double p = 1.0;
-#pragma unroll
-  for (int b = 0; b < 5; ++b) {
-    if ((n >> b) & 1) p *= lam;
-    lam *= lam;
-  }
-  return p;
-}
-
-__device__ double power_long(double lam, int64_t n) {
-  double p = 1.0;
-  for (; n > 0; n >>= 1) {
-    if (n & 1) p *= lam;
-    lam *= lam;
-  }
-  return p;
-}
 
 // four consecutive elements of a row from column col on, zero past the row's end (the single-step kernel)
 template <typename T>
@@ -88,381 +46,6 @@ __device__ __forceinline__ void load4(const T *row, int col, int dim, bool live,
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[e] = live && col + e < dim ? (float)row[col + e] : 0.f;
-  }
-}
-
-__device__ __forceinline__ bool not_finite(float v) { return !(__builtin_fabsf(v) <= 3.402823466e38f); }
-
-// ---- operands of the products.  `In` holds four values of k of an input, `Part` those of something computed in f32.
-// f32 (and f16, which f32 holds): four 16x16x4 products.
-struct Math32 {
-  typedef f32x4 In;
-  typedef f32x4 Part;
-  static __device__ __forceinline__ f32x4 mma(const f32x4 &a, const f32x4 &b, f32x4 c) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
-    return c;
-  }
-  static __device__ __forceinline__ Part split(const f32x4 &v) { return v; }
-  static __device__ __forceinline__ f32x4 mma_right(const In &a, const Part &b, f32x4 c) { return mma(a, b, c); }
-  static __device__ __forceinline__ f32x4 mma_left(const Part &a, const In &b, f32x4 c) { return mma(a, b, c); }
-  // s + b^T (w c)
-  static __device__ __forceinline__ In weigh(const In &c, const float (&w)[4]) {
-    return f32x4{c[0] * w[0], c[1] * w[1], c[2] * w[2], c[3] * w[3]};
-  }
-  static __device__ __forceinline__ f32x4 mma_state(const In &b, const In &wc, f32x4 s) { return mma(b, wc, s); }
-  static __device__ __forceinline__ float value(float v) { return v; }
-  static __device__ __forceinline__ bool bad(const In &v) {
-    return (int)not_finite(v[0]) | (int)not_finite(v[1]) | (int)not_finite(v[2]) | (int)not_finite(v[3]);
-  }
-};
-
-// bf16: one 16x16x16 product of the inputs as they are; what is computed in f32 goes in as a sum of bf16 parts, two of them
-// (relative error 2^-17, under a bf16 output's 2^-9) or three (2^-25) for the state, which is returned in f32.  (An infinite
-// value in f32 becomes inf + NaN: it stays not finite, but comes out as NaN.)
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
-
-struct Math16 {
-  typedef s16x4 In;
-  struct Part {
-    s16x4 hi, lo;
-  };
-  struct Part3 {
-    s16x4 hi, mid, lo;
-  };
-  static __device__ __forceinline__ f32x4 mma(const In &a, const In &b, const f32x4 &c) {
-    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ s16x4 round(const f32x4 &v) {
-    return __builtin_bit_cast(s16x4, __builtin_convertvector(v, b16x4));
-  }
-  static __device__ __forceinline__ f32x4 wide(const s16x4 &v) {
-    return __builtin_convertvector(__builtin_bit_cast(b16x4, v), f32x4);
-  }
-  static __device__ __forceinline__ Part split(const f32x4 &v) {
-    Part p;
-    p.hi = round(v);
-    p.lo = round(v - wide(p.hi));
-    return p;
-  }
-  static __device__ __forceinline__ f32x4 mma_right(const In &a, const Part &b, f32x4 c) {
-    return mma(a, b.hi, mma(a, b.lo, c));
-  }
-  static __device__ __forceinline__ f32x4 mma_left(const Part &a, const In &b, f32x4 c) {
-    return mma(a.hi, b, mma(a.lo, b, c));
-  }
-  static __device__ __forceinline__ Part3 weigh(const In &c, const float (&w)[4]) {
-    const f32x4 u = wide(c);
-    const f32x4 v = {u[0] * w[0], u[1] * w[1], u[2] * w[2], u[3] * w[3]};
-    Part3 p;
-    p.hi = round(v);
-    const f32x4 r = v - wide(p.hi);
-    p.mid = round(r);
-    p.lo = round(r - wide(p.mid));
-    return p;
-  }
-  static __device__ __forceinline__ f32x4 mma_state(const In &b, const Part3 &wc, f32x4 s) {
-    return mma(b, wc.hi, mma(b, wc.mid, mma(b, wc.lo, s)));
-  }
-  static __device__ __forceinline__ float value(short v) { return __uint_as_float((uint32_t)(uint16_t)v << 16); }
-  static __device__ __forceinline__ bool bad(const In &v) {
-    bool b = false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) b |= (v[e] & 0x7F80) == 0x7F80;
-    return b;
-  }
-};
-
-// ---- four consecutive elements of one step as they are loaded (`raw`: nothing touches them before their chunk's turn, so the
-// loads of a chunk fly while the one before it is worked on), and as they lie in LDS: bf16 as it is, the others in f32
-template <typename T>
-struct Quad {
-  typedef Math32 M;
-  typedef f32x4 Lds;
-  typedef float L;
-  uint32_t w[4];
-  template <bool VEC>
-  __device__ __forceinline__ Lds get() const {
-    if constexpr (sizeof(T) == 4) {
-      return f32x4{__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]), __uint_as_float(w[3])};
-    } else {
-      if constexpr (VEC) return f32x4{half(w[0]), half(w[0] >> 16), half(w[1]), half(w[1] >> 16)};
-      return f32x4{half(w[0]), half(w[1]), half(w[2]), half(w[3])};
-    }
-  }
-  static __device__ __forceinline__ float half(uint32_t u) { return (float)__builtin_bit_cast(trl_f16, (uint16_t)u); }
-};
-
-template <>
-struct Quad<trl_bf16> {
-  typedef Math16 M;
-  typedef s16x4 Lds;
-  typedef short L;
-  uint32_t w[4];
-  template <bool VEC>
-  __device__ __forceinline__ Lds get() const {
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(s16x4, VEC ? u32x2{w[0], w[1]} : u32x2{w[0] | (w[1] << 16), w[2] | (w[3] << 16)});
-  }
-};
-
-// `n`: elements of the quad that are inside the row and the chunk (0 .. 4; 0 or 4 with VEC); the others are not read, and zero
-// when the quad is staged
-template <typename T, bool VEC>
-__device__ __forceinline__ void fetch_quad(Quad<T> &q, const T *p, int n) {
-  typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type U;
-  if constexpr (VEC) {
-    if (n > 0) __builtin_memcpy(q.w, p, 4 * sizeof(T));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < n) q.w[e] = ((const U *)p)[e];
-  }
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ typename Quad<T>::Lds quad_of(const Quad<T> &q, int n) {
-  typename Quad<T>::Lds v = q.template get<VEC>();
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = (VEC ? n > 0 : e < n) ? v[e] : 0;
-  return v;
-}
-
-struct Scans {
-  Scan s[3];
-};
-
-constexpr int kColStride = 20;      // LDS: elements between two columns of a transposed tile (16 steps and 4 of padding)
-
-// LDS elements of one chunk: a and b by rows (16 steps of da + 4), b and c by columns
-template <int KT, bool OUT>
-__host__ __device__ constexpr int chunk_elems(int waves) {
-  return (OUT ? 2 * 16 * (16 * KT + 4) : 0) + (16 * KT + 16 * waves) * kColStride;
-}
-
-// A workgroup carries one (env, head, segment) of one of the scans (blockIdx.y) through time, a wave 16 of c's columns (waves
-// past them only help to stage).  KT: 16-column tiles of a's (b's) dimension, at most the workgroup's waves: every thread brings
-// one quad of a, of b and of c.  VEC: both dimensions are multiples of four.
-template <typename T, int KT, bool OUT, bool VEC>
-__global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
-  typedef typename Quad<T>::M M;
-  typedef typename Quad<T>::Lds V4;
-  typedef typename Quad<T>::L L;
-  constexpr int ROW = 16 * KT + 4;
-  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
-  __shared__ int bad_flag[2][8];
-  const Scan &s = all.s[blockIdx.y];
-  const int tid = threadIdx.x, waves = blockDim.x >> 6;
-  const int lane = tid & 63, x = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t heads = s.N * s.H;
-  const int64_t nh = blockIdx.x % heads;
-  // (the launch that makes contributions has no need of the last segment in its direction of time)
-  const int seg = (int)(blockIdx.x / heads) + (!OUT && s.reverse ? 1 : 0);
-  const int64_t n = nh / s.H;
-  const int h = (int)(nh % s.H);
-
-  const int64_t length = s.lengths ? std::min<int64_t>(std::max<int64_t>(s.lengths[n], 0), s.T) : s.T;
-  const int64_t t_lo = (int64_t)seg * s.seg_len;
-  const int64_t t_end = std::min<int64_t>(t_lo + s.seg_len, s.T);
-  const int64_t t_hi = std::min<int64_t>(t_end, length);      // steps [t_lo, t_hi) of this workgroup
-  const int steps = (int)std::max<int64_t>(t_hi - t_lo, 0);
-  const int64_t t_first = s.reverse ? t_hi - 1 : t_lo, dir = s.reverse ? -1 : 1;      // step i of the scan: t_first + dir i
-  const int off = s.reverse ? 0 : 1;
-  const int da = s.da, dc = s.dc;
-
-  // this thread's quads: step and column of a and b, step and column of c
-  const int arow = tid < 64 * KT ? tid / (4 * KT) : 16, acol = 4 * (tid % (4 * KT));
-  const int crow = tid / (4 * waves), ccol = 4 * (tid % (4 * waves));
-  const T *pa = (const T *)s.a.p + n * s.a.sn + h * s.a.sh + (t_first + dir * arow) * s.a.st + acol;
-  const T *pb = (const T *)s.b.p + n * s.b.sn + h * s.b.sh + (t_first + dir * arow) * s.b.st + acol;
-  const T *pc = (const T *)s.c.p + n * s.c.sn + h * s.c.sh + (t_first + dir * crow) * s.c.st + ccol;
-  const int64_t sa = 16 * dir * s.a.st, sb = 16 * dir * s.b.st, sc = 16 * dir * s.c.st;
-
-  Quad<T> qa = {}, qb = {}, qc = {};
-  float flag = 0.f;
-  auto fetch = [&](int done, int m) {      // the next chunk, of m steps; advances the pointers
-    const int na = arow < m ? da - acol : 0, nc = crow < m ? dc - ccol : 0;
-    if constexpr (OUT) fetch_quad<T, VEC>(qa, pa, na);
-    fetch_quad<T, VEC>(qb, pb, na);
-    fetch_quad<T, VEC>(qc, pc, nc);
-    pa += sa, pb += sb, pc += sc;
-    if (s.start != nullptr && x < m) {
-      const int64_t at = (t_first + dir * (done + x)) * s.N + n;
-      flag = s.start_u8 ? (float)((const uint8_t *)s.start)[at] : ((const float *)s.start)[at];
-    }
-  };
-  auto lds = [&](int buf) { return (L *)lds_raw + buf * chunk_elems<KT, OUT>(waves); };
-  // the chunk's m steps (one < 0), or its step `one` alone as the first of a chunk of its own
-  auto stage = [&](int buf, int m, int one) {
-    L *A = lds(buf), *B = A + (OUT ? 16 * ROW : 0), *BT = B + (OUT ? 16 * ROW : 0), *CT = BT + 16 * KT * kColStride;
-    bool bad = false;
-    if (KT >= 8 || tid < 64 * KT) {
-      const int na = (one < 0 ? arow < m : arow == one) ? da - acol : 0, row = one < 0 ? arow : (arow - one) & 15;
-      if constexpr (OUT) *(V4 *)(A + row * ROW + acol) = quad_of<T, VEC>(qa, na);
-      const V4 v = quad_of<T, VEC>(qb, na);
-      if constexpr (OUT) *(V4 *)(B + row * ROW + acol) = v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) BT[(acol + e) * kColStride + row] = v[e];
-      bad = M::bad(v);
-    }
-    const int nc = (one < 0 ? crow < m : crow == one) ? dc - ccol : 0, row = one < 0 ? crow : (crow - one) & 15;
-    const V4 v = quad_of<T, VEC>(qc, nc);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) CT[(ccol + e) * kColStride + row] = v[e];
-    bad = __any((int)bad | (int)M::bad(v));
-    if (lane == 0) bad_flag[buf][wave] = bad;
-  };
-
-  if (steps > 0) fetch(0, std::min(16, steps));
-
-  const int ccolx = wave * 16 + x;      // this lane's column of c, of S and of the output
-  f32x4 S[KT];
-  {
-    // state entering the segment: the caller's, or the joined contributions of the segments before it
-    const float *in = s.seg_state ? s.seg_state + (nh * s.segs + seg) * da * dc : s.state_in;
-    if (s.seg_state == nullptr && in != nullptr) in += nh * da * dc;
-    const int64_t rs = s.state_t ? 1 : dc, cs = s.state_t ? da : 1;
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = kt * 16 + 4 * g + r;
-        S[kt][r] = 0.f;
-        if (OUT && in != nullptr) {
-          const float v = in[std::min(row, da - 1) * rs + std::min(ccolx, dc - 1) * cs];
-          S[kt][r] = ((row < da) & (ccolx < dc)) ? v : 0.f;
-        }
-      }
-  }
-
-  const double lam = (double)s.decay[h];
-  float w_intra[4], w_inter[4], w_state[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int j = 4 * g + r;
-    w_intra[r] = j <= x ? (float)power(lam, x - j) * s.s_intra : 0.f;
-    w_inter[r] = (float)power(lam, j + off) * s.s_inter;
-    w_state[r] = (float)power(lam, 16 - off - j) * s.s_state;
-  }
-  const double full = power(lam, 16);
-  const float full_hi = (float)full, full_lo = (float)(full - (double)full_hi);
-
-  bool cut = false;            // a start inside this segment
-  int chunk = std::min(16, steps), buf = 0, one = -1;
-#pragma unroll 1
-  for (int begin = 0; begin < steps; buf ^= 1) {
-    stage(buf, chunk, one);
-    uint32_t F = 0;            // bit i: step i of the chunk is a start
-    if (s.start != nullptr) F = (uint32_t)__ballot((flag != 0.f) & (lane < chunk));
-    // one barrier a chunk: the other buffer is written only after every wave has passed this one
-    __syncthreads();
-    const bool any_bad = __any(bad_flag[buf][std::min(lane, waves - 1)]);
-    if (any_bad && chunk > 1 && one < 0) {
-      // b or c holds an infinity or a NaN, which a weight of zero would spread over the chunk: its steps one at a time
-      one = 0;
-      continue;
-    }
-    const int m = one < 0 ? chunk : 1, done = begin + std::max(one, 0);
-    if (one >= 0) F = (F >> one) & 1;
-    cut |= F != 0;
-    if (one < 0 || one == chunk - 1) {
-      begin += chunk;
-      chunk = std::min(16, steps - begin);
-      one = -1;
-      if (begin < steps) fetch(begin, chunk);
-    } else {
-      ++one;
-    }
-    const L *A = lds(buf), *B = A + (OUT ? 16 * ROW : 0), *BT = B + (OUT ? 16 * ROW : 0),
-            *CT = BT + 16 * KT * kColStride;
-    const V4 C = *(const V4 *)(CT + ccolx * kColStride + 4 * g);
-    if constexpr (OUT) {
-      f32x4 P = {0.f, 0.f, 0.f, 0.f}, o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const V4 av = *(const V4 *)(A + x * ROW + kt * 16 + 4 * g), bv = *(const V4 *)(B + x * ROW + kt * 16 + 4 * g);
-        P = M::mma(bv, av, P);
-        o = M::mma_right(av, M::split(S[kt]), o);
-      }
-      f32x4 p;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = 4 * g + r;
-        const uint32_t le_j = (1u << (j + off)) - 1, le_x = (1u << (x + off)) - 1;
-        const bool on = (j <= x) & ((F & le_x & ~le_j) == 0);
-        p[r] = on ? P[r] * w_intra[r] : 0.f;
-        o[r] = (F & le_j) == 0 ? o[r] * w_inter[r] : 0.f;
-      }
-      o = M::mma_left(M::split(p), C, o);
-      T *po = (T *)s.out + ((t_first + dir * (done + 4 * g)) * heads + nh) * dc + ccolx;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if ((4 * g + r < m) & (ccolx < dc)) po[r * dir * heads * dc] = (T)o[r];
-    }
-    float hi = full_hi, lo = full_lo, ws[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) ws[e] = w_state[e];
-    if (m != 16) {
-      const double pm = power(lam, m);
-      hi = (float)pm;
-      lo = (float)(pm - (double)hi);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) ws[e] = (float)power(lam, std::max(m - off - (4 * g + e), 0)) * s.s_state;
-    }
-    // steps that a start keeps from the chunk's end weigh nothing (b and c are finite, or this is one step alone)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) ws[e] = (F & ~((1u << (4 * g + e + off)) - 1)) == 0 ? ws[e] : 0.f;
-    if (F != 0) {
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) S[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    } else {
-      // (lambda^m in two parts: its rounding would otherwise repeat in the same direction every chunk)
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[kt][r] = fmaf(S[kt][r], hi, S[kt][r] * lo);
-    }
-    // (one step alone whose own start cuts it off -- backward in time -- leaves nothing, whatever c holds)
-    if (!any_bad || off == 1 || F == 0) {
-      const auto wc = M::weigh(C, ws);
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const V4 bt = *(const V4 *)(BT + (kt * 16 + x) * kColStride + 4 * g);
-        S[kt] = M::mma_state(bt, wc, S[kt]);
-      }
-    }
-    if (any_bad) {             // rows past da: 0 times a value that is not finite
-      int rows = da - 4 * g;
-      asm volatile("" : "+v"(rows));      // (its comparisons are made here, not kept over the loop)
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (kt * 16 + r >= rows) S[kt][r] = 0.f;
-    }
-  }
-
-  // the state left behind: the caller's at the end of time, or this segment's contribution
-  float *left = nullptr;
-  if (!OUT) {
-    left = s.seg_state + (nh * s.segs + seg) * da * dc;
-    if (tid == 0) s.seg_coef[nh * s.segs + seg] = cut ? -1.f : (float)power_long(lam, steps);
-  } else if (s.state_out != nullptr && seg == (s.reverse ? 0 : s.segs - 1)) {
-    left = s.state_out + nh * da * dc;
-  }
-  if (left != nullptr) {
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = kt * 16 + 4 * g + r;
-        if ((row < da) & (ccolx < dc)) left[(int64_t)row * dc + ccolx] = S[kt][r];
-      }
-  }
-  if (OUT) {                   // steps past the sequence's end
-    for (int64_t t = std::max<int64_t>(t_lo, length) + g; t < t_end; t += 4)
-      if (ccolx < dc) ((T *)s.out)[(t * heads + nh) * dc + ccolx] = (T)0.f;
   }
 }
 
@@ -538,8 +121,6 @@ __global__ __launch_bounds__(kThreads) void k_step(const T *__restrict__ q, cons
   }
 }
 
-int tiles_of(int dim) { return (dim + 15) / 16; }
-
 // time segments: enough workgroups to fill the chip, of at least 64 steps each
 void segments(int64_t T, int64_t heads, int *segs, int *seg_len) {
   int64_t want = heads > 0 ? trl_cdiv(512, heads) : 1;
@@ -549,43 +130,13 @@ void segments(int64_t T, int64_t heads, int *segs, int *seg_len) {
   *segs = (int)std::max<int64_t>(1, trl_cdiv(T, len));
 }
 
-template <typename T, int KT, bool OUT, bool VEC>
-void scan_launch_k(const Scans &s, dim3 grid, int waves, hipStream_t st) {
-  const size_t bytes = (size_t)2 * chunk_elems<KT, OUT>(waves) * sizeof(typename Quad<T>::L);
-  if (bytes > 48 * 1024)      // (per device and cheap; a refusal shows at the launch)
-    (void)hipFuncSetAttribute((const void *)k_scan<T, KT, OUT, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  k_scan<T, KT, OUT, VEC><<<grid, 64 * waves, bytes, st>>>(s);
-}
-
-template <typename T, bool OUT, bool VEC>
-void scan_launch_t(const Scans &s, int kt, dim3 grid, int waves, hipStream_t st) {
-  switch (kt) {
-    case 1: return scan_launch_k<T, 1, OUT, VEC>(s, grid, waves, st);
-    case 2: return scan_launch_k<T, 2, OUT, VEC>(s, grid, waves, st);
-    case 3: return scan_launch_k<T, 3, OUT, VEC>(s, grid, waves, st);
-    case 4: return scan_launch_k<T, 4, OUT, VEC>(s, grid, waves, st);
-    case 5: return scan_launch_k<T, 5, OUT, VEC>(s, grid, waves, st);
-    case 6: return scan_launch_k<T, 6, OUT, VEC>(s, grid, waves, st);
-    default: return scan_launch_k<T, 8, OUT, VEC>(s, grid, waves, st);      // (7 tiles too)
-  }
-}
-
-// `count` scans of equal sizes in one launch
 void scan_launch(const Scans &all, int count, int32_t dtype, bool out, hipStream_t st) {
-  const Scan &f = all.s[0];
-  const dim3 grid((unsigned)(f.N * f.H * (out ? f.segs : f.segs - 1)), count);
-  const int kt = tiles_of(f.da), waves = std::max(kt == 7 ? 8 : kt, tiles_of(f.dc));
-  const bool vec = f.da % 4 == 0 && f.dc % 4 == 0;
-  TRL_FOR_DTYPE(dtype, {
-    if (out && vec)
-      scan_launch_t<T, true, true>(all, kt, grid, waves, st);
-    else if (out)
-      scan_launch_t<T, true, false>(all, kt, grid, waves, st);
-    else if (vec)
-      scan_launch_t<T, false, true>(all, kt, grid, waves, st);
-    else
-      scan_launch_t<T, false, false>(all, kt, grid, waves, st);
-  });
+  if (dtype == TRL_F32)
+    launch_f32(all, count, out, st);
+  else if (dtype == TRL_BF16)
+    launch_bf16(all, count, out, st);
+  else
+    launch_f16(all, count, out, st);
 }
 
 void join_launch(const Scan &s, hipStream_t st) {
