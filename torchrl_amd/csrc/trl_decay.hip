@@ -50,15 +50,16 @@ __device__ __forceinline__ void load4(const T *row, int col, int dim, bool live,
 }
 
 // seg_state[s]: contribution of segment s -> state entering segment s, in the scan's direction.  coef < 0: a start in it.
-__global__ __launch_bounds__(kThreads) void k_join(float *__restrict__ seg_state, const float *__restrict__ seg_coef,
-                                                   const float *__restrict__ state_in, int64_t heads, int64_t size,
-                                                   int segs, int reverse) {
+// blockIdx.y: one of the scans.
+__global__ __launch_bounds__(kThreads) void k_join(Scans all, int64_t heads, int64_t size) {
+  const Scan &s = all.s[blockIdx.y];
   const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (e >= heads * size) return;
   const int64_t nh = e / size;
-  float *p = seg_state + nh * segs * size + (e - nh * size);
-  const float *coef = seg_coef + nh * segs;
-  float cur = state_in ? state_in[e] : 0.f;
+  const int segs = s.segs, reverse = s.reverse;
+  float *p = s.seg_state + nh * segs * size + (e - nh * size);
+  const float *coef = s.seg_coef + nh * segs;
+  float cur = s.state_in ? s.state_in[e] : 0.f;
   const int first = reverse ? segs - 1 : 0, dir = reverse ? -1 : 1;
   for (int i0 = 0; i0 < segs; i0 += 8) {
     float u[8], cf[8];         // eight contributions in flight
@@ -125,6 +126,7 @@ __global__ __launch_bounds__(kThreads) void k_step(const T *__restrict__ q, cons
 void segments(int64_t T, int64_t heads, int *segs, int *seg_len) {
   int64_t want = heads > 0 ? trl_cdiv(512, heads) : 1;
   want = std::max<int64_t>(1, std::min<int64_t>(want, T / 64));
+  if (want < 3) want = 1;
   const int64_t len = std::max<int64_t>(16, trl_cdiv(trl_cdiv(T, want), 16) * 16);
   *seg_len = (int)len;
   *segs = (int)std::max<int64_t>(1, trl_cdiv(T, len));
@@ -139,10 +141,17 @@ void scan_launch(const Scans &all, int count, int32_t dtype, bool out, hipStream
     launch_f16(all, count, out, st);
 }
 
-void join_launch(const Scan &s, hipStream_t st) {
-  const int64_t heads = s.N * s.H, size = (int64_t)s.da * s.dc;
-  k_join<<<(int)trl_cdiv(heads * size, kThreads), kThreads, 0, st>>>(s.seg_state, s.seg_coef, s.state_in, heads, size, s.segs,
-                                                                    s.reverse);
+// the contributions of `count` scans of equal sizes, and their join where the workgroups do not make it themselves
+int contributions(const char *fn, const Scans &all, int count, int32_t dtype, hipStream_t st) {
+  scan_launch(all, count, dtype, false, st);
+  TRL_CHECK_LAUNCH(fn);
+  const Scan &f = all.s[0];
+  if (f.segs > kJoinInside) {
+    const int64_t heads = f.N * f.H, size = (int64_t)f.da * f.dc;
+    k_join<<<dim3((unsigned)trl_cdiv(heads * size, kThreads), count), kThreads, 0, st>>>(all, heads, size);
+    TRL_CHECK_LAUNCH(fn);
+  }
+  return TRL_OK;
 }
 
 int decay_check(const char *fn, int64_t T, int64_t N, int32_t H, int32_t dk, int32_t dv, int32_t dtype) {
@@ -206,10 +215,7 @@ extern "C" int trl_decay_attention_fwd(const void *q, const void *k, const void 
     TRL_REQUIRE(workspace != nullptr, "%s: null workspace", fn);
     s.seg_state = (float *)workspace;
     s.seg_coef = s.seg_state + N * H * s.segs * (int64_t)dk * dv;
-    scan_launch(Scans{{s}}, 1, dtype, false, st);
-    TRL_CHECK_LAUNCH(fn);
-    join_launch(s, st);
-    TRL_CHECK_LAUNCH(fn);
+    if (int rc = contributions(fn, Scans{{s}}, 1, dtype, st)) return rc;
   }
   scan_launch(Scans{{s}}, 1, dtype, true, st);
   TRL_CHECK_LAUNCH(fn);
@@ -271,11 +277,7 @@ extern "C" int trl_decay_attention_bwd(const void *gy, const float *gstate, cons
     f.seg_coef = ws_s + coef;
     r.seg_state = ws_r;
     r.seg_coef = ws_r + coef;
-    scan_launch(Scans{{f, r}}, 2, dtype, false, st);
-    TRL_CHECK_LAUNCH(fn);
-    join_launch(f, st);
-    join_launch(r, st);
-    TRL_CHECK_LAUNCH(fn);
+    if (int rc = contributions(fn, Scans{{f, r}}, 2, dtype, st)) return rc;
   }
   // dv: (k, q, do) backward in time; its last state is the gradient of the initial one
   r.out = dv_out;

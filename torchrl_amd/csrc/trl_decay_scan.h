@@ -38,6 +38,10 @@ void launch_f32(const Scans &all, int count, bool out, hipStream_t st);
 void launch_bf16(const Scans &all, int count, bool out, hipStream_t st);
 void launch_f16(const Scans &all, int count, bool out, hipStream_t st);
 
+// up to so many segments a workgroup joins the contributions before its own by itself: 2 us at 8 of them, against 7 us and a
+// launch for the join of all; beyond, what all workgroups read grows with the square of the segments
+constexpr int kJoinInside = 8;
+
 inline int tiles_of(int dim) { return (dim + 15) / 16; }
 
 // lambda^n in double, n < 32: each power is rounded to f32 once
@@ -69,6 +73,7 @@ __device__ __forceinline__ bool not_finite(float v) { return !(__builtin_fabsf(v
 // ---- operands of the products.  `In` holds four values of k of an input, `Part` those of something computed in f32.
 // f32 (and f16, which f32 holds): four 16x16x4 products.
 struct Math32 {
+  static constexpr bool kShare = true;
   typedef f32x4 In;
   typedef f32x4 Part;
   static __device__ __forceinline__ f32x4 mma(const f32x4 &a, const f32x4 &b, f32x4 c) {
@@ -97,6 +102,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
 
 struct Math16 {
+  static constexpr bool kShare = false;
   typedef s16x4 In;
   struct Part {
     s16x4 hi, lo;
@@ -210,14 +216,19 @@ __device__ __forceinline__ int col_at(int col, int row) {
   return col * kColStride + ((((row >> 2) ^ (col >> 4)) & 3) << 2) + (row & 3);
 }
 
-// LDS bytes: two chunks -- a by rows (16 steps of da + 4), b and c by columns -- and the parts of the pair products
-template <typename L, int KT, bool OUT>
+// LDS: two chunks -- a by rows (16 steps of da + 4), b and c by columns -- and, for the pair products, either their parts
+// (kShare) or b by rows too.
+// Every wave needs all pair products.  In f32 they would be a third of its matrix instructions (16 of 52 a chunk at 64
+// columns), so each wave makes the part of one tile of columns and the parts are added through LDS, behind a second barrier:
+// 677 -> 592 us for a training pass over 256 steps of 2,048 heads.  On the bf16 MFMA all of them cost 4 instructions of half
+// the length, less than the exchange takes.
+template <typename T, int KT, bool OUT>
 __host__ __device__ constexpr int chunk_elems(int waves) {
-  return (OUT ? 16 * (16 * KT + 4) : 0) + (16 * KT + 16 * waves) * kColStride;
+  return (OUT ? (Quad<T>::M::kShare ? 1 : 2) * 16 * (16 * KT + 4) : 0) + (16 * KT + 16 * waves) * kColStride;
 }
-template <typename L, int KT, bool OUT>
+template <typename T, int KT, bool OUT>
 constexpr int lds_bytes(int waves) {
-  return 2 * chunk_elems<L, KT, OUT>(waves) * (int)sizeof(L) + (OUT ? KT * 1024 : 0);
+  return 2 * chunk_elems<T, KT, OUT>(waves) * (int)sizeof(typename Quad<T>::L) + (OUT && Quad<T>::M::kShare ? KT * 1024 : 0);
 }
 
 // A workgroup carries one (env, head, segment) of one of the scans (blockIdx.y) through time, a wave 16 of c's columns (waves
@@ -231,6 +242,7 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
   constexpr int ROW = 16 * KT + 4;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   __shared__ int bad_flag[2][8];
+  __shared__ float pw[48], pw_lo[32];
   const Scan &s = all.s[blockIdx.y];
   const int tid = threadIdx.x, waves = blockDim.x >> 6;
   const int lane = tid & 63, x = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -256,133 +268,186 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
   const T *pa = (const T *)s.a.p + n * s.a.sn + h * s.a.sh + (t_first + dir * arow) * s.a.st + acol;
   const T *pb = (const T *)s.b.p + n * s.b.sn + h * s.b.sh + (t_first + dir * arow) * s.b.st + acol;
   const T *pc = (const T *)s.c.p + n * s.c.sn + h * s.c.sh + (t_first + dir * crow) * s.c.st + ccol;
-  const int64_t sa = 16 * dir * s.a.st, sb = 16 * dir * s.b.st, sc = 16 * dir * s.c.st;
+  const int64_t sa = dir * s.a.st, sb = dir * s.b.st, sc = dir * s.c.st;
 
-  Quad<T> qa = {}, qb = {}, qc = {};
-  float flag = 0.f;
-  auto fetch = [&](int done, int m) {      // the next chunk, of m steps; advances the pointers
+  struct Quads {
+    Quad<T> a, b, c;
+    float flag;                // of step x
+  };
+  auto fetch = [&](Quads &q, int at) {      // the chunk that begins with step `at` (none past the end)
+    const int m = steps - at;
     const int na = arow < m ? da - acol : 0, nc = crow < m ? dc - ccol : 0;
-    if constexpr (OUT) fetch_quad<T, VEC>(qa, pa, na);
-    fetch_quad<T, VEC>(qb, pb, na);
-    fetch_quad<T, VEC>(qc, pc, nc);
-    pa += sa, pb += sb, pc += sc;
+    if constexpr (OUT) fetch_quad<T, VEC>(q.a, pa + at * sa, na);
+    fetch_quad<T, VEC>(q.b, pb + at * sb, na);
+    fetch_quad<T, VEC>(q.c, pc + at * sc, nc);
     if (s.start != nullptr && x < m) {
-      const int64_t at = (t_first + dir * (done + x)) * s.N + n;
-      flag = s.start_u8 ? (float)((const uint8_t *)s.start)[at] : ((const float *)s.start)[at];
+      const int64_t i = (t_first + dir * (at + x)) * s.N + n;
+      q.flag = s.start_u8 ? (float)((const uint8_t *)s.start)[i] : ((const float *)s.start)[i];
     }
   };
-  auto lds = [&](int buf) { return (L *)lds_raw + buf * chunk_elems<L, KT, OUT>(waves); };
-  f32x4 *const parts = (f32x4 *)((L *)lds_raw + 2 * chunk_elems<L, KT, OUT>(waves));
+  auto lds = [&](int buf) { return (L *)lds_raw + buf * chunk_elems<T, KT, OUT>(waves); };
+  f32x4 *const parts = (f32x4 *)((L *)lds_raw + 2 * chunk_elems<T, KT, OUT>(waves));
   // the chunk's m steps (one < 0), or its step `one` alone as the first of a chunk of its own; whether b or c is not finite
-  auto stage = [&](int buf, int m, int one) {
-    L *A = lds(buf), *BT = A + (OUT ? 16 * ROW : 0), *CC = BT + 16 * KT * kColStride;
+  auto stage = [&](const Quads &q, int buf, int m, int one) {
+    L *A = lds(buf), *B = A + 16 * ROW, *BT = A + (OUT ? (M::kShare ? 1 : 2) * 16 * ROW : 0), *CC = BT + 16 * KT * kColStride;
     bool bad = false;
     if (arow < 16) {
       const int na = (one < 0 ? arow < m : arow == one) ? da - acol : 0, row = one < 0 ? arow : (arow - one) & 15;
-      if constexpr (OUT) *(V4 *)(A + row * ROW + acol) = quad_of<T, VEC>(qa, na);
-      const V4 v = quad_of<T, VEC>(qb, na);
+      if constexpr (OUT) *(V4 *)(A + row * ROW + acol) = quad_of<T, VEC>(q.a, na);
+      const V4 v = quad_of<T, VEC>(q.b, na);
+      if constexpr (OUT && !M::kShare) *(V4 *)(B + row * ROW + acol) = v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) BT[col_at(acol, row) + e * kColStride] = v[e];
       bad = M::bad(v);
     }
     const int nc = (one < 0 ? crow < m : crow == one) ? dc - ccol : 0, row = one < 0 ? crow : (crow - one) & 15;
-    const V4 v = quad_of<T, VEC>(qc, nc);
+    const V4 v = quad_of<T, VEC>(q.c, nc);
 #pragma unroll
     for (int e = 0; e < 4; ++e) CC[col_at(ccol, row) + e * kColStride] = v[e];
     return (bool)((int)bad | (int)M::bad(v));
   };
 
-  if (steps > 0) fetch(0, std::min(16, steps));
+  Quads q = {};
+  fetch(q, 0);
 
   const int col = wave * 16 + x;      // this lane's column of c, of S and of the output
   f32x4 S[KT];
   {
-    // state entering the segment: the caller's, or the joined contributions of the segments before it; none: zero.  Every lane
-    // loads from an address inside it (from decay's first where there is none) and nothing branches: with a branch per value
-    // the compiler carries all of S through each of them and spills
-    const float *in = s.seg_state ? s.seg_state + (nh * s.segs + seg) * da * dc : s.state_in;
-    if (s.seg_state == nullptr && in != nullptr) in += nh * da * dc;
-    const bool have = OUT && in != nullptr;
-    if (!have) in = s.decay;
-    const int rs = have ? (s.state_t ? 1 : dc) : 0, cs = have ? (s.state_t ? da : 1) : 0;
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = kt * 16 + 4 * g + r;
-        const float v = OUT ? in[std::min(row, da - 1) * rs + std::min(col, dc - 1) * cs] : 0.f;
-        S[kt][r] = ((int)have & (int)(row < da) & (int)(col < dc)) ? v : 0.f;
+    // state entering the segment, none: zero.  Every lane loads from an address inside it (from decay's first where there is
+    // none) and no value has a branch of its own: through each of those the compiler would carry all of S, and spill
+    const int64_t size = (int64_t)da * dc;
+    const float *in = s.state_in ? s.state_in + nh * size : nullptr;
+    int first = 0, joins = 0;      // contributions still to be joined: segments first, first + dir, ..
+    if (s.seg_state != nullptr) {
+      if (s.segs > kJoinInside) {
+        in = s.seg_state + (nh * s.segs + seg) * size;      // (joined by the launch before)
+      } else {
+        first = s.reverse ? s.segs - 1 : 0;
+        joins = s.reverse ? s.segs - 1 - seg : seg;
       }
-      __builtin_amdgcn_sched_barrier(0);      // (the addresses of all of them do not fit beside S)
+    }
+    const bool have = OUT && in != nullptr;
+    // a state from memory, in S's layout.  Four rows of a column lie side by side when it is read transposed.
+    auto load_state = [&](const float *p, bool live, f32x4 (&v)[KT]) {
+      if (VEC && s.state_t) {
+        p += live ? (int64_t)std::min(col, dc - 1) * da : 0;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+          if (live) __builtin_memcpy(&v[kt], p + std::min(kt * 16 + 4 * g, da - 4), 16);
+      } else {
+        const int rs = live ? (s.state_t ? 1 : dc) : 0, cs = live ? (s.state_t ? da : 1) : 0;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[kt][r] = p[std::min(kt * 16 + 4 * g + r, da - 1) * rs + std::min(col, dc - 1) * cs];
+          __builtin_amdgcn_sched_barrier(0);      // (the addresses of all of them do not fit beside S)
+        }
+      }
+    };
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) S[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (OUT) {
+      load_state(have ? in : s.decay, have, S);
+      f32x4 u[KT];
+      const float *p = s.seg_state + (nh * s.segs + first) * size, *pc = s.seg_coef + nh * s.segs + first;
+      if (joins > 0) load_state(p, true, u);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[kt][r] = ((int)have & (int)(kt * 16 + 4 * g + r < da) & (int)(col < dc)) ? S[kt][r] : 0.f;
+#pragma unroll 1
+      for (int i = 0; i < joins; ++i) {
+        const float cf = pc[(int)dir * i];      // < 0: a start in that segment
+        f32x4 next[KT];
+        p += dir * size;
+        if (i + 1 < joins) load_state(p, true, next);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float w = cf < 0.f ? u[kt][r] : fmaf(cf, S[kt][r], u[kt][r]);
+            S[kt][r] = ((int)(kt * 16 + 4 * g + r < da) & (int)(col < dc)) ? w : 0.f;
+          }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) u[kt] = next[kt];
+      }
     }
   }
 
+  // the powers of lambda, by one thread each and to one rounding; zero below the 0th, so that steps after a chunk's end weigh
+  // nothing
   const double lam = (double)s.decay[h];
-  float w_intra[4], w_inter[4], w_state[4];
+  if (tid < 32) {
+    const double p = power(lam, tid);
+    pw[16 + tid] = (float)p;
+    pw_lo[tid] = (float)(p - (double)(float)p);
+    if (tid < 16) pw[tid] = 0.f;
+  }
+  __syncthreads();
+  float w_intra[4], w_inter[4], w_state[4];      // of a whole chunk
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const int j = 4 * g + r;
-    w_intra[r] = j <= x ? (float)power(lam, x - j) * s.s_intra : 0.f;
-    w_inter[r] = (float)power(lam, j + off) * s.s_inter;
-    w_state[r] = (float)power(lam, 16 - off - j) * s.s_state;
+    w_intra[r] = pw[16 + x - 4 * g - r] * s.s_intra;
+    w_inter[r] = pw[16 + off + 4 * g + r] * s.s_inter;
+    w_state[r] = pw[32 - off - 4 * g - r] * s.s_state;
   }
-  const double full = power(lam, 16);
-  const float full_hi = (float)full, full_lo = (float)(full - (double)full_hi);
+  const float full_hi = pw[32], full_lo = pw_lo[16];
 
   const int64_t out_step = dir * heads * dc;
   T *po = OUT ? (T *)s.out + ((t_first + dir * 4 * g) * heads + nh) * dc + col : nullptr;      // step 4 g of the chunk
   bool cut = false;            // a start inside this segment
-  int chunk = std::min(16, steps), buf = 0, one = -1;
+  int buf = 0;
 #pragma unroll 1
-  for (int begin = 0; begin < steps; buf ^= 1) {
-    bool any_bad = __any(stage(buf, chunk, one));
-    uint32_t F = 0;            // bit i: step i of the chunk is a start
-    if (s.start != nullptr) F = (uint32_t)__ballot((flag != 0.f) & (lane < chunk));
-    if (lane == 0) bad_flag[buf][wave] = any_bad;
+  for (int begin = 0, one = -1; begin < steps; buf ^= 1) {
+    const int chunk = std::min(16, steps - begin);
+    const bool bad = __any(stage(q, buf, chunk, one));
+    uint32_t F = 0;          // bit i: step i of the chunk is a start
+    if (s.start != nullptr) F = (uint32_t)__ballot((q.flag != 0.f) & (lane < chunk));
+    if (one >= 0) F = (F >> one) & 1;
+    if (lane == 0) bad_flag[buf][wave] = bad;
     // the other buffer is written only after every wave has passed this barrier
     __syncthreads();
-    any_bad = __any(bad_flag[buf][std::min(lane, waves - 1)]);
-    if (any_bad && chunk > 1 && one < 0) {
-      // b or c holds an infinity or a NaN, which a weight of zero would spread over the chunk: its steps one at a time
-      one = 0;
-      continue;
-    }
-    const int m = one < 0 ? chunk : 1;
-    if (one >= 0) F = (F >> one) & 1;
-    cut |= F != 0;
-    if (one < 0 || one == chunk - 1) {
-      begin += chunk;
-      chunk = std::min(16, steps - begin);
-      one = -1;
-      if (begin < steps) fetch(begin, chunk);
-    } else {
-      ++one;
-    }
-    const L *A = lds(buf), *BT = A + (OUT ? 16 * ROW : 0), *CC = BT + 16 * KT * kColStride;
+    const int bad_any = bad_flag[buf][std::min(lane, waves - 1)];
+    if (one < 0 || one == chunk - 1) fetch(q, begin + 16);      // on its way while this chunk is worked on
+    const L *A = lds(buf), *B = A + 16 * ROW, *BT = A + (OUT ? (M::kShare ? 1 : 2) * 16 * ROW : 0),
+            *CC = BT + 16 * KT * kColStride;
     const V4 C = *(const V4 *)(CC + col_at(col, 4 * g));
+    f32x4 P = {0.f, 0.f, 0.f, 0.f}, o = {0.f, 0.f, 0.f, 0.f};
     if constexpr (OUT) {
-      // pair products b a^T: every wave would need all of them, so each makes the part of one tile of columns
-      if (wave < KT) {
+      if (M::kShare && wave < KT) {
         const V4 av = *(const V4 *)(A + x * ROW + wave * 16 + 4 * g);
         V4 bv;
 #pragma unroll
         for (int e = 0; e < 4; ++e) bv[e] = BT[col_at(wave * 16 + 4 * g + e, x)];
-        parts[wave * 64 + lane] = M::mma(bv, av, f32x4{0.f, 0.f, 0.f, 0.f});
+        parts[wave * 64 + lane] = M::mma(bv, av, P);
       }
-      f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
         const V4 av = *(const V4 *)(A + x * ROW + kt * 16 + 4 * g);
+        if constexpr (!M::kShare) P = M::mma(*(const V4 *)(B + x * ROW + kt * 16 + 4 * g), av, P);
         o = M::mma_right(av, M::split(S[kt]), o);
       }
-      if (KT > 1 || waves > 1) __syncthreads();      // (written again only after the next chunk's first barrier)
-      f32x4 P = parts[lane];
+      if constexpr (M::kShare) {
+        if (KT > 1 || waves > 1) __syncthreads();      // (written again only after the next chunk's first barrier)
+        P = parts[lane];
 #pragma unroll
-      for (int kt = 1; kt < KT; ++kt) {
-        const f32x4 q = parts[kt * 64 + lane];
+        for (int kt = 1; kt < KT; ++kt) {
+          const f32x4 part = parts[kt * 64 + lane];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) P[r] += q[r];
+          for (int r = 0; r < 4; ++r) P[r] += part[r];
+        }
       }
+    }
+    const bool any_bad = __any(bad_any);
+    if (any_bad && chunk > 1 && one < 0) {
+      // b or c holds an infinity or a NaN, which a weight of zero would spread over the chunk: its steps one at a time
+      one = 0;
+      fetch(q, begin);
+      continue;
+    }
+    const int m = one < 0 ? chunk : 1;
+    cut |= F != 0;
+    if constexpr (OUT) {
       f32x4 p;
       if (F == 0) {
 #pragma unroll
@@ -410,11 +475,9 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) ws[e] = w_state[e];
     if (m != 16) {
-      const double pm = power(lam, m);
-      hi = (float)pm;
-      lo = (float)(pm - (double)hi);
+      hi = pw[16 + m], lo = pw_lo[m];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ws[e] = (float)power(lam, std::max(m - off - (4 * g + e), 0)) * s.s_state;
+      for (int e = 0; e < 4; ++e) ws[e] = pw[16 + m - off - 4 * g - e] * s.s_state;
     }
     if (F != 0) {
       // steps that a start keeps from the chunk's end weigh nothing (b and c are finite, or this is one step alone)
@@ -447,6 +510,10 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
         for (int r = 0; r < 4; ++r)
           if (kt * 16 + r >= rows) S[kt][r] = 0.f;
     }
+    if (one < 0 || ++one == chunk) {
+      begin += chunk;
+      one = -1;
+    }
   }
 
   // the state left behind: the caller's at the end of time, or this segment's contribution
@@ -475,7 +542,7 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
 template <typename T, int KT, bool OUT, bool VEC>
 void launch_k(const Scans &s, dim3 grid, hipStream_t st) {
   const int waves = std::max(KT, tiles_of(s.s[0].dc));
-  const int bytes = lds_bytes<typename Quad<T>::L, KT, OUT>(waves);
+  const int bytes = lds_bytes<T, KT, OUT>(waves);
   if (bytes > 48 * 1024)      // (per device and cheap; a refusal shows at the launch)
     (void)hipFuncSetAttribute((const void *)k_scan<T, KT, OUT, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   k_scan<T, KT, OUT, VEC><<<grid, 64 * waves, bytes, st>>>(s);

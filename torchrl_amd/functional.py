@@ -589,6 +589,12 @@ def _beside(t, other, what):
   return t
 
 
+def _first_order(backward):
+  """torch.autograd.function.once_differentiable at no cost where no graph of the gradients is asked for."""
+  strict = torch.autograd.function.once_differentiable(backward)
+  return lambda ctx, *grads: strict(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+
 class _LayerNorm(torch.autograd.Function):
   @staticmethod
   def forward(ctx, x, weight, bias, eps, act):
@@ -608,7 +614,7 @@ class _LayerNorm(torch.autograd.Function):
     return y
 
   @staticmethod
-  @torch.autograd.function.once_differentiable
+  @_first_order
   def backward(ctx, gy):
     x, weight, bias, stats = ctx.saved_tensors
     rows, width, lib = ctx.rows, ctx.width, _lib.lib()
@@ -670,7 +676,7 @@ class _Dropout(torch.autograd.Function):
                            call_d)
 
   @staticmethod
-  @torch.autograd.function.once_differentiable
+  @_first_order
   def backward(ctx, gy):
     code, p, seed, call = ctx.args
     call_d, = ctx.saved_tensors
@@ -791,7 +797,7 @@ class _DecayAttention(torch.autograd.Function):
     return out, last
 
   @staticmethod
-  @torch.autograd.function.once_differentiable
+  @_first_order
   def backward(ctx, gy, glast):
     q, k, v, state, decay, start, lengths = ctx.saved_tensors
     start_code, scale = ctx.args
