@@ -68,8 +68,6 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ bool not_finite(float v) { return !(__builtin_fabsf(v) <= 3.402823466e38f); }
-
 // ---- operands of the products.  `In` holds four values of k of an input, `Part` those of something computed in f32.
 // f32 (and f16, which f32 holds): four 16x16x4 products.
 struct Math32 {
@@ -90,9 +88,9 @@ struct Math32 {
     return f32x4{c[0] * w[0], c[1] * w[1], c[2] * w[2], c[3] * w[3]};
   }
   static __device__ __forceinline__ f32x4 mma_state(const In &b, const In &wc, f32x4 s) { return mma(b, wc, s); }
-  static __device__ __forceinline__ bool bad(const In &v) {
-    return (int)not_finite(v[0]) | (int)not_finite(v[1]) | (int)not_finite(v[2]) | (int)not_finite(v[3]);
-  }
+  // not zero where a value is not finite (0 times it is a NaN)
+  static __device__ __forceinline__ float doubt(const In &v) { return v[0] * 0.f + v[1] * 0.f + (v[2] * 0.f + v[3] * 0.f); }
+  static __device__ __forceinline__ bool bad(float doubt) { return doubt != 0.f; }
 };
 
 // bf16: one 16x16x16 product of the inputs as they are; what is computed in f32 goes in as a sum of bf16 parts, two of them
@@ -144,12 +142,13 @@ struct Math16 {
   static __device__ __forceinline__ f32x4 mma_state(const In &b, const Weighed &wc, f32x4 s) {
     return mma(b, wc.hi, mma(b, wc.mid, mma(b, wc.lo, s)));
   }
-  static __device__ __forceinline__ bool bad(const In &v) {
-    bool b = false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) b |= (v[e] & 0x7F80) == 0x7F80;
-    return b;
+  // bit 15 or 31 where an exponent is all ones
+  static __device__ __forceinline__ uint32_t doubt(const In &v) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 u = __builtin_bit_cast(u32x2, v);
+    return ((u[0] & 0x7F807F80u) + 0x00800080u) | ((u[1] & 0x7F807F80u) + 0x00800080u);
   }
+  static __device__ __forceinline__ bool bad(uint32_t doubt) { return (doubt & 0x80008000u) != 0; }
 };
 
 // ---- four consecutive elements of one step as they are loaded (`raw`: nothing touches them before their chunk's turn, so the
@@ -270,6 +269,10 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
   const T *pc = (const T *)s.c.p + n * s.c.sn + h * s.c.sh + (t_first + dir * crow) * s.c.st + ccol;
   const int64_t sa = dir * s.a.st, sb = dir * s.b.st, sc = dir * s.c.st;
 
+  // Every quad of a whole chunk is inside its operand: nothing to select when it is staged.  Where that is worth code of its own:
+  // bf16 with the usual sizes (256 steps of 256 heads of 64: 80 -> 74 us; f32 loses 4% to the longer loop).
+  constexpr bool kWhole = VEC && !M::kShare && (KT & (KT - 1)) == 0;
+  const bool whole = kWhole && waves == KT && da == 16 * KT && dc == 16 * KT;
   struct Quads {
     Quad<T> a, b, c;
     float flag;                // of step x
@@ -290,21 +293,25 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
   // the chunk's m steps (one < 0), or its step `one` alone as the first of a chunk of its own; whether b or c is not finite
   auto stage = [&](const Quads &q, int buf, int m, int one) {
     L *A = lds(buf), *B = A + 16 * ROW, *BT = A + (OUT ? (M::kShare ? 1 : 2) * 16 * ROW : 0), *CC = BT + 16 * KT * kColStride;
-    bool bad = false;
-    if (arow < 16) {
-      const int na = (one < 0 ? arow < m : arow == one) ? da - acol : 0, row = one < 0 ? arow : (arow - one) & 15;
-      if constexpr (OUT) *(V4 *)(A + row * ROW + acol) = quad_of<T, VEC>(q.a, na);
-      const V4 v = quad_of<T, VEC>(q.b, na);
-      if constexpr (OUT && !M::kShare) *(V4 *)(B + row * ROW + acol) = v;
+    auto put = [&](V4 a, V4 b, V4 c, int ra, int rc) {
+      if (KT >= 8 || arow < 16) {
+        if constexpr (OUT) *(V4 *)(A + ra * ROW + acol) = a;
+        if constexpr (OUT && !M::kShare) *(V4 *)(B + ra * ROW + acol) = b;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) BT[col_at(acol, row) + e * kColStride] = v[e];
-      bad = M::bad(v);
+        for (int e = 0; e < 4; ++e) BT[col_at(acol, ra) + e * kColStride] = b[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) CC[col_at(ccol, rc) + e * kColStride] = c[e];
+    };
+    if (kWhole && whole && m == 16 && one < 0) {
+      const V4 b = q.b.template get<true>(), c = q.c.template get<true>();
+      put(q.a.template get<true>(), b, c, arow, crow);
+      return (int)M::bad(M::doubt(b)) | (int)M::bad(M::doubt(c));
     }
-    const int nc = (one < 0 ? crow < m : crow == one) ? dc - ccol : 0, row = one < 0 ? crow : (crow - one) & 15;
-    const V4 v = quad_of<T, VEC>(q.c, nc);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) CC[col_at(ccol, row) + e * kColStride] = v[e];
-    return (bool)((int)bad | (int)M::bad(v));
+    const int na = (one < 0 ? arow < m : arow == one) ? da - acol : 0, nc = (one < 0 ? crow < m : crow == one) ? dc - ccol : 0;
+    const V4 b = quad_of<T, VEC>(q.b, arow < 16 ? na : 0), c = quad_of<T, VEC>(q.c, nc);
+    put(quad_of<T, VEC>(q.a, na), b, c, one < 0 ? arow : (arow - one) & 15, one < 0 ? crow : (crow - one) & 15);
+    return (int)M::bad(M::doubt(b)) | (int)M::bad(M::doubt(c));
   };
 
   Quads q = {};
@@ -400,7 +407,7 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
 #pragma unroll 1
   for (int begin = 0, one = -1; begin < steps; buf ^= 1) {
     const int chunk = std::min(16, steps - begin);
-    const bool bad = __any(stage(q, buf, chunk, one));
+    const bool bad = __any(stage(q, buf, chunk, one) != 0);
     uint32_t F = 0;          // bit i: step i of the chunk is a start
     if (s.start != nullptr) F = (uint32_t)__ballot((q.flag != 0.f) & (lane < chunk));
     if (one >= 0) F = (F >> one) & 1;
@@ -466,9 +473,14 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
         }
       }
       o = M::mma_left(M::split(p), C, o);
+if (m == 16 && dc == 16 * waves) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if ((4 * g + r < m) & (col < dc)) po[r * out_step] = (T)o[r];
+        for (int r = 0; r < 4; ++r) po[r * out_step] = (T)o[r];
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if ((4 * g + r < m) & (col < dc)) po[r * out_step] = (T)o[r];
+      }
       po += m * out_step;
     }
     float hi = full_hi, lo = full_lo, ws[4];
