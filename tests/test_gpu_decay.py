@@ -479,3 +479,16 @@ def test_memory_block_dropout_and_bf16():
   y.float().sum().backward()
   assert y.dtype == torch.bfloat16 and s.dtype == torch.float32
   assert all(torch.isfinite(p.grad).all() for p in h.parameters())
+
+
+def test_second_derivatives_are_refused_and_library_errors_keep_their_class():
+  from torchrl_amd import _lib
+  x = torch.randn(4, 8, device=DEV, requires_grad=True)
+  for y in (F.layer_norm(x), F.dropout(x, 0.5, 1, 2),
+            F.decay_attention(x.view(4, 1, 1, 8), x.view(4, 1, 1, 8), x.view(4, 1, 1, 8), torch.ones(1, device=DEV))[0]):
+    g, = torch.autograd.grad(y.square().sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError, match='differentiate twice'):
+      g.sum().backward()
+  q = torch.empty(1, 1 << 22, 1, 1, device=DEV)
+  with pytest.raises(_lib.TrlError, match='too many'):
+    F.decay_attention(q, q, q, torch.ones(1, device=DEV))

@@ -21,6 +21,9 @@ LIB_PATH = os.path.join(LIB_DIR, 'libtrl_hip.so')
 # that tools/*_sweep.py drive through environment variables (TRL_GAE_TUNE, TRL_GATHER_*, TRL_MLP_DBG,
 # TRL_U8_FWD_WGS).  The production library above contains none of them and never reads the environment.
 TUNE_LIB_PATH = os.path.join(LIB_DIR, 'libtrl_hip_tune.so')
+# Graph nodes of the layer functions for torch's engine (a Python extension; host code, built with g++ against torch's headers)
+AUTOGRAD_PATH = os.path.join(LIB_DIR, 'trl_autograd.so')
+AUTOGRAD_SOURCE = 'trl_autograd.cpp'
 SOURCES = ['trl_host.cpp', 'trl_replay.hip', 'trl_gae.hip', 'trl_loss.hip', 'trl_mlp.hip', 'trl_learn.hip',
            'trl_offpolicy.hip', 'trl_linear_u8.hip', 'trl_act.hip', 'trl_epoch.hip', 'trl_norm.hip', 'trl_decay.hip',
            'trl_decay_f32.hip', 'trl_decay_bf16.hip', 'trl_decay_f16.hip']
@@ -49,7 +52,28 @@ def is_stale(tuning=False):
     return True
   t = os.path.getmtime(lib)
   deps = [os.path.join(CSRC, s) for s in SOURCES] + HEADERS
-  return any(os.path.getmtime(d) > t for d in deps)
+  if any(os.path.getmtime(d) > t for d in deps):
+    return True
+  if tuning:
+    return False
+  if not os.path.exists(AUTOGRAD_PATH):
+    return True
+  t = os.path.getmtime(AUTOGRAD_PATH)
+  return any(os.path.getmtime(d) > t for d in (os.path.join(CSRC, AUTOGRAD_SOURCE), os.path.join(ROOT, 'include', 'trl_hip.h')))
+
+
+def _autograd_command():
+  import sysconfig
+  import torch
+  from torch.utils import cpp_extension
+  cmd = [shutil.which('g++') or 'g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-Wall',
+         '-D_GLIBCXX_USE_CXX11_ABI=%d' % int(torch._C._GLIBCXX_USE_CXX11_ABI), '-I', os.path.join(ROOT, 'include')]
+  for path in cpp_extension.include_paths() + [sysconfig.get_paths()['include']]:
+    cmd += ['-isystem', path]
+  cmd += [os.path.join(CSRC, AUTOGRAD_SOURCE), '-o', AUTOGRAD_PATH]
+  for path in cpp_extension.library_paths():
+    cmd += ['-L' + path, '-Wl,-rpath,' + path]
+  return cmd + ['-lc10', '-ltorch_cpu', '-ltorch', '-ltorch_python']
 
 
 def build_library(force=False, verbose=True, tuning=False):
@@ -75,10 +99,15 @@ def build_library(force=False, verbose=True, tuning=False):
       print(' '.join(cmd), flush=True)
     procs.append((s, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
     objs.append(obj)
+  if not tuning:
+    cmd = _autograd_command()
+    if verbose:
+      print(' '.join(cmd), flush=True)
+    procs.append((AUTOGRAD_SOURCE, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
   for s, p in procs:
     out, _ = p.communicate()
     if p.returncode != 0:
-      raise RuntimeError('hipcc failed on %s:\n%s' % (s, out.decode(errors='replace')))
+      raise RuntimeError('the compiler failed on %s:\n%s' % (s, out.decode(errors='replace')))
     if verbose and out.strip():
       print(out.decode(errors='replace'))
   cmd = [hipcc, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', lib_path] + objs

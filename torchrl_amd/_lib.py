@@ -181,6 +181,29 @@ def lib():
   return _lib
 
 
+_nodes = None
+
+
+def nodes():
+  """The graph nodes of the layer functions (lib/trl_autograd.so, csrc/trl_autograd.cpp), bound to the loaded library's entry
+  points; raises with a build hint if the extension is not there."""
+  global _nodes
+  if _nodes is None:
+    import importlib.util
+    handle = lib()
+    path = os.path.join(_PKG, 'lib', 'trl_autograd.so')
+    if not os.path.exists(path):
+      raise TrlError('%s not found: build it with `python -m torchrl_amd._build`' % path)
+    spec = importlib.util.spec_from_file_location('trl_autograd', path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    module.bind([C.cast(getattr(handle, n), C.c_void_p).value for n in (
+        'trl_last_error', 'trl_layer_norm_fwd', 'trl_layer_norm_bwd_workspace_bytes', 'trl_layer_norm_bwd', 'trl_dropout',
+        'trl_decay_attention_workspace_bytes', 'trl_decay_attention_fwd', 'trl_decay_attention_bwd')], TrlError)
+    _nodes = module
+  return _nodes
+
+
 def check(rc):
   if rc != 0:
     raise TrlError('libtrl_hip error %d: %s' % (rc, lib().trl_last_error().decode(errors='replace')))

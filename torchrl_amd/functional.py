@@ -3,10 +3,9 @@
 Every function here takes device tensors and enqueues kernels on torch's current stream.
 There is no CPU implementation behind any of them: a CPU tensor raises TrlError.
 The loss functions are autograd Functions whose forward runs the fused kernel (loss AND
-its backward seeds in one pass) and whose backward only scales the saved seeds.
+its backward seeds in one pass) and whose backward only scales the saved seeds.  Layer norm, dropout and
+decay attention have their graph nodes in native code (csrc/trl_autograd.cpp); their arguments are checked here.
 """
-import ctypes as C
-
 import torch
 
 from . import _lib
@@ -589,50 +588,6 @@ def _beside(t, other, what):
   return t
 
 
-def _first_order(backward):
-  """torch.autograd.function.once_differentiable at no cost where no graph of the gradients is asked for."""
-  strict = torch.autograd.function.once_differentiable(backward)
-  return lambda ctx, *grads: strict(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-
-
-class _LayerNorm(torch.autograd.Function):
-  @staticmethod
-  def forward(ctx, x, weight, bias, eps, act):
-    code = _LAYER_DTYPES[x.dtype]
-    x = x.contiguous()
-    width = x.shape[-1]
-    rows = x.numel() // width
-    y = torch.empty_like(x)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad) else None
-    with _lib.device_guard(x.device):
-      _lib.check(_lib.lib().trl_layer_norm_fwd(
-          x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), rows, width, code, eps, act, y.data_ptr(),
-          stats.data_ptr() if stats is not None else None, stats.data_ptr() + 4 * rows if stats is not None else None,
-          _lib.stream_ptr(x.device)))
-    ctx.code, ctx.act, ctx.rows, ctx.width = code, act, rows, width
-    ctx.save_for_backward(x, weight, bias, stats)
-    return y
-
-  @staticmethod
-  @_first_order
-  def backward(ctx, gy):
-    x, weight, bias, stats = ctx.saved_tensors
-    rows, width, lib = ctx.rows, ctx.width, _lib.lib()
-    need_x, need_w, need_b = ctx.needs_input_grad[:3]
-    gy = gy.contiguous()
-    dx = torch.empty_like(x) if need_x else None
-    dw = torch.empty_like(weight) if need_w else None
-    db = torch.empty_like(bias) if need_b else None
-    ws = None
-    if need_w or need_b:      # (a buffer of this call alone: two streams or two captured graphs never share one)
-      ws = torch.empty(lib.trl_layer_norm_bwd_workspace_bytes(rows, width, ctx.code), dtype=torch.uint8, device=x.device)
-    with _lib.device_guard(x.device):
-      _lib.check(lib.trl_layer_norm_bwd(gy.data_ptr(), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), stats.data_ptr(),
-                                        stats.data_ptr() + 4 * rows, rows, width, ctx.code, ctx.act, _lib.ptr(dx),
-                                        _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), _lib.stream_ptr(x.device)))
-    return dx, dw, db, None, None
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False):
   """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension (then ReLU), torch.nn.functional.layer_norm's
   definition; one HIP launch forward, two backward (csrc/trl_norm.hip).
@@ -655,33 +610,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False):
       if t.dtype != torch.float32 or not t.is_contiguous():
         t = t.float().contiguous()
     params.append(t)
-  return _LayerNorm.apply(x, params[0], params[1], eps, 1 if relu else 0)
-
-
-def _dropout_launch(x, residual, code, p, seed, call, call_d):
-  y = torch.empty_like(x)
   with _lib.device_guard(x.device):
-    _lib.check(_lib.lib().trl_dropout(x.data_ptr(), _lib.ptr(residual), x.numel(), code, p, seed, call, _lib.ptr(call_d),
-                                      y.data_ptr(), _lib.stream_ptr(x.device)))
-  return y
-
-
-class _Dropout(torch.autograd.Function):
-  @staticmethod
-  def forward(ctx, x, residual, p, seed, call, call_d):
-    code = _LAYER_DTYPES[x.dtype]
-    ctx.args = code, p, seed, call
-    ctx.save_for_backward(call_d)      # (written to since: autograd refuses the backward pass)
-    return _dropout_launch(x.contiguous(), residual.contiguous() if residual is not None else None, code, p, seed, call,
-                           call_d)
-
-  @staticmethod
-  @_first_order
-  def backward(ctx, gy):
-    code, p, seed, call = ctx.args
-    call_d, = ctx.saved_tensors
-    gx = _dropout_launch(gy.contiguous(), None, code, p, seed, call, call_d) if ctx.needs_input_grad[0] else None
-    return gx, gy if ctx.needs_input_grad[1] else None, None, None, None, None
+    return _lib.nodes().layer_norm(x, params[0], params[1], eps, 1 if relu else 0, _lib.stream_ptr(x.device))
 
 
 def dropout(x, p, seed, call, residual=None):
@@ -711,7 +641,8 @@ def dropout(x, p, seed, call, residual=None):
     if residual.shape != x.shape or residual.dtype != x.dtype:
       raise ValueError('dropout: residual must be %s %s like x, got %s %s' %
                        (tuple(x.shape), x.dtype, tuple(residual.shape), residual.dtype))
-  return _Dropout.apply(x, residual, p, int(seed) & (2 ** 64 - 1), int(call), call_d)
+  with _lib.device_guard(x.device):
+    return _lib.nodes().dropout(x, residual, p, int(seed) & (2 ** 64 - 1), int(call), call_d, _lib.stream_ptr(x.device))
 
 
 def next_call(counter):
@@ -773,52 +704,6 @@ def _dense_heads(t):
   return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
 
 
-def _scan_strides(q, k, v):
-  return (C.c_int64 * 9)(*(q.stride()[:3] + k.stride()[:3] + v.stride()[:3]))
-
-
-class _DecayAttention(torch.autograd.Function):
-  @staticmethod
-  def forward(ctx, q, k, v, state, decay, start, lengths, start_code, scale):
-    T, N, H, dk = q.shape
-    dv, code, lib = v.shape[3], _LAYER_DTYPES[q.dtype], _lib.lib()
-    out = torch.empty((T, N, H, dv), dtype=q.dtype, device=q.device)
-    last = torch.empty((N, H, dk, dv), dtype=torch.float32, device=q.device)
-    nbytes = lib.trl_decay_attention_workspace_bytes(T, N, H, dk, dv, 0)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-    with _lib.device_guard(q.device):
-      _lib.check(lib.trl_decay_attention_fwd(
-          q.data_ptr(), k.data_ptr(), v.data_ptr(), _scan_strides(q, k, v), decay.data_ptr(), _lib.ptr(start), start_code,
-          _lib.ptr(lengths), _lib.ptr(state), T, N, H, dk, dv, code, scale, out.data_ptr(), last.data_ptr(), _lib.ptr(ws),
-          _lib.stream_ptr(q.device)))
-    ctx.set_materialize_grads(False)
-    ctx.args = start_code, scale
-    ctx.save_for_backward(q, k, v, state, decay, start, lengths)
-    return out, last
-
-  @staticmethod
-  @_first_order
-  def backward(ctx, gy, glast):
-    q, k, v, state, decay, start, lengths = ctx.saved_tensors
-    start_code, scale = ctx.args
-    T, N, H, dk = q.shape
-    dv, code, lib = v.shape[3], _LAYER_DTYPES[q.dtype], _lib.lib()
-    gy = torch.zeros((T, N, H, dv), dtype=q.dtype, device=q.device) if gy is None else gy.contiguous()
-    glast = glast.contiguous() if glast is not None else None
-    gq = torch.empty((T, N, H, dk), dtype=q.dtype, device=q.device)
-    gk = torch.empty_like(gq)
-    gv = torch.empty_like(gy)
-    gs = torch.empty((N, H, dk, dv), dtype=torch.float32, device=q.device) if ctx.needs_input_grad[3] else None
-    nbytes = lib.trl_decay_attention_workspace_bytes(T, N, H, dk, dv, 1)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-    with _lib.device_guard(q.device):
-      _lib.check(lib.trl_decay_attention_bwd(
-          gy.data_ptr(), _lib.ptr(glast), q.data_ptr(), k.data_ptr(), v.data_ptr(), _scan_strides(q, k, v), decay.data_ptr(),
-          _lib.ptr(start), start_code, _lib.ptr(lengths), _lib.ptr(state), T, N, H, dk, dv, code, scale, gq.data_ptr(),
-          gk.data_ptr(), gv.data_ptr(), _lib.ptr(gs), _lib.ptr(ws), _lib.stream_ptr(q.device)))
-    return gq, gk, gv, gs, None, None, None, None, None
-
-
 def decay_attention(q, k, v, decay, scale=None, start=None, lengths=None, state=None):
   """Linear attention with a decay per head over a rollout [T, N, .] (csrc/trl_decay.hip): the sequence form of a memory
   whose single-step form is decay_attention_step.  For every env and head, with S a [Dk, Dv] matrix,
@@ -845,8 +730,10 @@ def decay_attention(q, k, v, decay, scale=None, start=None, lengths=None, state=
     _state_like(fn, state, q, (N, H, dk, v.shape[3]))
     state = state.contiguous()
   scale = dk ** -0.5 if scale is None else float(scale)
-  return _DecayAttention.apply(_dense_heads(q), _dense_heads(k), _dense_heads(v), state, decay.contiguous(), start, lengths,
-                               start_code, scale)
+  with _lib.device_guard(q.device):
+    out, last = _lib.nodes().decay_attention(_dense_heads(q), _dense_heads(k), _dense_heads(v), state, decay.contiguous(), start,
+                                             lengths, start_code, scale, _lib.stream_ptr(q.device))
+  return out, last
 
 
 def decay_attention_step(q, k, v, decay, state, scale=None, start=None, out_state=None):
