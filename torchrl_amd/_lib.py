@@ -199,7 +199,8 @@ def nodes():
     spec.loader.exec_module(module)
     module.bind([C.cast(getattr(handle, n), C.c_void_p).value for n in (
         'trl_last_error', 'trl_layer_norm_fwd', 'trl_layer_norm_bwd_workspace_bytes', 'trl_layer_norm_bwd', 'trl_dropout',
-        'trl_decay_attention_workspace_bytes', 'trl_decay_attention_fwd', 'trl_decay_attention_bwd')], TrlError)
+        'trl_decay_attention_workspace_bytes', 'trl_decay_attention_fwd', 'trl_decay_attention_bwd',
+        'trl_decay_attention_step')], TrlError)
     _nodes = module
   return _nodes
 

@@ -30,6 +30,7 @@ struct Api {
   decltype(&trl_decay_attention_workspace_bytes) decay_ws;
   decltype(&trl_decay_attention_fwd) decay_fwd;
   decltype(&trl_decay_attention_bwd) decay_bwd;
+  decltype(&trl_decay_attention_step) decay_step;
 } api;
 
 // a call the library refused: _lib.TrlError in Python (out of a backward pass the engine makes it a RuntimeError, its base)
@@ -227,6 +228,18 @@ std::vector<Tensor> decay_attention(const Tensor &q, const Tensor &k, const Tens
   return decay_run(q, k, v, get(state), decay, get(start), get(lengths), start_code, scale, stream);
 }
 
+// (no gradients; out_state may be state)
+std::vector<Tensor> decay_step(const Tensor &q0, const Tensor &k0, const Tensor &v0, const Tensor &decay, const Maybe &start,
+                               int64_t start_code, const Tensor &state, const Maybe &out_state, double scale, int64_t stream) {
+  const Tensor q = q0.contiguous(), k = k0.contiguous(), v = v0.contiguous();
+  Tensor out = at::empty(v.sizes(), v.options()), next = out_state ? *out_state : at::empty(state.sizes(), state.options());
+  check(api.decay_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), fptr(decay), ptr(get(start)), (int32_t)start_code, fptr(state),
+                       q.size(0), (int32_t)q.size(1), (int32_t)q.size(2), (int32_t)v.size(2), dtype_of(q), scale, out.data_ptr(),
+                       fptr(next), (void *)stream));
+  if (out_state) next.unsafeGetTensorImpl()->bump_version();      // (a graph that saved it as it was refuses its backward pass)
+  return {out, next};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(trl_autograd, m) {
@@ -241,4 +254,5 @@ PYBIND11_MODULE(trl_autograd, m) {
   m.def("layer_norm", &layer_norm);
   m.def("dropout", &dropout);
   m.def("decay_attention", &decay_attention);
+  m.def("decay_step", &decay_step);
 }

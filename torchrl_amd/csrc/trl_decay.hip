@@ -61,17 +61,17 @@ __global__ __launch_bounds__(kThreads) void k_join(Scans all, int64_t heads, int
   const float *coef = s.seg_coef + nh * segs;
   float cur = s.state_in ? s.state_in[e] : 0.f;
   const int first = reverse ? segs - 1 : 0, dir = reverse ? -1 : 1;
-  for (int i0 = 0; i0 < segs; i0 += 8) {
-    float u[8], cf[8];         // eight contributions in flight
+  for (int i0 = 0; i0 < segs; i0 += 16) {
+    float u[16], cf[16];       // sixteen contributions in flight
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 16; ++i) {
       const bool on = i0 + i < segs - 1;      // (the last one moves nothing on)
       const int sg = first + dir * (i0 + i);
       u[i] = on ? p[sg * size] : 0.f;
       cf[i] = on ? coef[sg] : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 16; ++i) {
       if (i0 + i < segs) p[(first + dir * (i0 + i)) * size] = cur;
       cur = cf[i] < 0.f ? u[i] : fmaf(cf[i], cur, u[i]);
     }

@@ -492,7 +492,9 @@ extern "C" int trl_layer_norm_bwd(const void *gy, const void *x, const float *we
 // is at least p 2^32: the mask of a call is a function of (seed, c, i) alone, so the backward pass makes it again instead of
 // reading it, and a call on a part of the memory or on another grid keeps the same elements.  (The top bit keeps the
 // counters apart from those of the exploration draws, csrc/trl_act.hip, under an equal seed.)
-// Bound by memory in float32; the generator costs 20 32 x 32 -> 64 bit products for four elements.
+// The generator costs 18 32 x 32 -> 64 bit products a lane for four elements (two of its 20 are the same for a whole wave).  In
+// float32 and with a residual that hides behind the memory (1M x 64 bf16 + residual: 84 us, 4.8 TB/s, a copy's rate); bf16 in and
+// out without one is bound by them (65 us, 4.1 TB/s; a slot more in flight made it 76).
 namespace {
 
 __device__ __forceinline__ void philox4(uint64_t seed, uint64_t call, uint32_t group, uint32_t group_hi, uint32_t (&c)[4]) {
@@ -501,9 +503,16 @@ __device__ __forceinline__ void philox4(uint64_t seed, uint64_t call, uint32_t g
   c[2] = group;
   c[3] = group_hi | 0x80000000u;
   uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+  // (philox_round of trl_common.h with both exclusive ors of a word in one instruction)
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
-    philox_round(c, k0, k1);
+    const uint64_t p0 = (uint64_t)0xD2511F53u * c[0], p1 = (uint64_t)0xCD9E8D57u * c[2];
+    const uint32_t n0 = __builtin_amdgcn_bitop3_b32((uint32_t)(p1 >> 32), c[1], k0, 0x96);
+    const uint32_t n2 = __builtin_amdgcn_bitop3_b32((uint32_t)(p0 >> 32), c[3], k1, 0x96);
+    c[1] = (uint32_t)p1;
+    c[3] = (uint32_t)p0;
+    c[0] = n0;
+    c[2] = n2;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }

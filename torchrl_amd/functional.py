@@ -751,9 +751,7 @@ def decay_attention_step(q, k, v, decay, state, scale=None, start=None, out_stat
     raise ValueError('%s has no gradient: call it under torch.no_grad(), or decay_attention with T = 1' % fn)
   given = state
   state = state.contiguous()
-  if out_state is None:
-    out_state = torch.empty(shape, dtype=torch.float32, device=q.device)
-  else:
+  if out_state is not None:
     _state_like(fn, out_state, q, shape, 'out_state')
     if not out_state.is_contiguous():
       raise ValueError('%s: out_state must be contiguous' % fn)
@@ -764,14 +762,11 @@ def decay_attention_step(q, k, v, decay, state, scale=None, start=None, out_stat
       raise ValueError('%s: out_state overlaps state without being it' % fn)
     if state is not given and out_state.untyped_storage().data_ptr() == given.untyped_storage().data_ptr():
       raise ValueError('%s: out_state shares memory with a state that is not contiguous' % fn)
-  out = torch.empty((N, H, dv), dtype=q.dtype, device=q.device)
   scale = dk ** -0.5 if scale is None else float(scale)
-  q, k, v, decay = q.contiguous(), k.contiguous(), v.contiguous(), decay.contiguous()
   with _lib.device_guard(q.device):
-    _lib.check(_lib.lib().trl_decay_attention_step(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), _lib.ptr(start), start_code, state.data_ptr(), N, H, dk,
-        dv, code, scale, out.data_ptr(), out_state.data_ptr(), _lib.stream_ptr(q.device)))
-  return out, out_state
+    out, state = _lib.nodes().decay_step(q, k, v, decay.contiguous(), start, start_code, state, out_state, scale,
+                                         _lib.stream_ptr(q.device))
+  return out, state if out_state is None else out_state
 
 
 def _fill_desc(d, weights, biases):
