@@ -56,8 +56,13 @@ def layer_norm(x, w, b, eps, relu, gy=None):
 # ------------------------------------------------------------------------------ dropout
 def philox_words(n, seed, call):
   """Word i % 4 of Philox-4x32-10, key = seed, counter = (call, i // 4 with its top bit set), for i < n."""
+  return philox_words_from(0, n, seed, call)
+
+
+def philox_words_from(first, n, seed, call):
+  """The same for first <= i < first + n, first a multiple of 4."""
   low = 0xFFFFFFFF
-  groups = np.arange((n + 3) // 4, dtype=np.uint64)
+  groups = np.arange((n + 3) // 4, dtype=np.uint64) + np.uint64(first // 4)
   c = [np.full_like(groups, call & low), np.full_like(groups, call >> 32), groups & np.uint64(low),
        (groups >> np.uint64(32)) | np.uint64(1 << 31)]
   k = [seed & low, seed >> 32]

@@ -198,13 +198,14 @@ def _same_pattern(got, want, bound, what):
   assert over.numel() == 0 or float(over.max()) <= 0, what
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('value', [float('nan'), float('inf'), -float('inf')])
 @pytest.mark.parametrize('T,where', [(60, 21), (700, 333)])
 @pytest.mark.parametrize('name', ['q', 'k', 'v'])
-def test_decay_attention_not_finite_steps_reach_only_what_they_touch(name, T, where, value):
+def test_decay_attention_not_finite_steps_reach_only_what_they_touch(name, T, where, value, dtype):
   """A value that is not finite changes the steps of its own episode from its own on, in its env and head, and nothing else:
   not the steps before it (which share its chunk), not those behind the next start."""
-  a = _inputs(T, 2, 2, 20, 24, cuts=0.0)
+  a = _inputs(T, 2, 2, 20, 24, dtype=dtype)
   a['start'] = torch.zeros(T, 2)
   a['start'][[where - 8, where + 9], 0] = 1.0
   clean = dict(a)
@@ -212,7 +213,7 @@ def test_decay_attention_not_finite_steps_reach_only_what_they_touch(name, T, wh
   a[name][where, 0, 1, 3] = value
   kw = dict(start=a['start'], state=a['state'])
   want = ref.decay_attention(a['q'], a['k'], a['v'], a['decay'], **kw)
-  bound = ref.decay_bounds(clean['q'], clean['k'], clean['v'], clean['decay'], torch.float32, **kw)
+  bound = ref.decay_bounds(clean['q'], clean['k'], clean['v'], clean['decay'], dtype, **kw)
   got = _run(a, grads=False)
   for n in ('out', 'state'):
     _same_pattern(got[n], want[n], bound[n], n)
@@ -220,14 +221,15 @@ def test_decay_attention_not_finite_steps_reach_only_what_they_touch(name, T, wh
   assert not torch.isfinite(want['out'][where, 0, 1]).all()
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('T,where', [(60, 21), (700, 333)])
 @pytest.mark.parametrize('name', ['q', 'k', 'v', 'gy'])
-def test_decay_attention_gradients_of_not_finite_steps(name, T, where):
-  a = _inputs(T, 2, 2, 20, 24)
+def test_decay_attention_gradients_of_not_finite_steps(name, T, where, dtype):
+  a = _inputs(T, 2, 2, 20, 24, dtype=dtype)
   a['start'] = torch.zeros(T, 2)
   a['start'][[where - 8, where + 9], 0] = 1.0
   kw = dict(start=a['start'], state=a['state'], gy=a['gy'], gstate=a['gstate'])
-  bound = ref.decay_bounds(a['q'], a['k'], a['v'], a['decay'], torch.float32, **kw)
+  bound = ref.decay_bounds(a['q'], a['k'], a['v'], a['decay'], dtype, **kw)
   a = dict(a, **{name: a[name].clone()})
   a[name][where, 0, 1, 3] = float('nan')
   kw['gy'] = a['gy']
@@ -295,15 +297,17 @@ def test_decay_attention_same_bits_every_run(shape):
       assert torch.equal(runs[0][n], r[n]), n
 
 
-def test_decay_attention_captured_and_on_other_streams():
-  a = _inputs(700, 1, 2, 32, 32, cuts=0.01)      # (in segments: the captured passes bring workspaces of their own)
+@pytest.mark.parametrize('D', [32, 128])
+def test_decay_attention_captured_and_on_other_streams(D):
+  a = _inputs(700, 1, 2, D, D, cuts=0.01)      # (in segments: the captured passes bring workspaces of their own)
   dev = {n: (t.to(DEV) if t is not None else None) for n, t in a.items()}
   for n in ('q', 'k', 'v'):
     dev[n].requires_grad_(True)
 
   def body():
     out, s = F.decay_attention(dev['q'], dev['k'], dev['v'], dev['decay'], start=dev['start'], state=dev['state'])
-    return (out, s) + torch.autograd.grad(out, [dev['q'], dev['k'], dev['v']], dev['gy'])
+    # (no graph outlives the body)
+    return (out.detach(), s.detach()) + torch.autograd.grad(out, [dev['q'], dev['k'], dev['v']], dev['gy'])
 
   side = torch.cuda.Stream()
   side.wait_stream(torch.cuda.current_stream())
@@ -492,3 +496,37 @@ def test_second_derivatives_are_refused_and_library_errors_keep_their_class():
   q = torch.empty(1, 1 << 22, 1, 1, device=DEV)
   with pytest.raises(_lib.TrlError, match='too many'):
     F.decay_attention(q, q, q, torch.ones(1, device=DEV))
+
+
+def test_decay_attention_offsets_past_32_bits():
+  """Steps 60 M elements apart: the last ones lie past 2^31 elements and 2^32 bytes."""
+  T, N, H, D = 40, 2, 2, 32
+  a = _inputs(T, N, H, D, D, dtype=torch.bfloat16, cuts=0.05)
+  base = _run(a)
+  stride = 60_000_000
+  far = {}
+  for n in ('q', 'k', 'v'):
+    buf = torch.empty((T - 1) * stride + N * H * D, dtype=torch.bfloat16, device=DEV)
+    far[n] = buf.as_strided((T, N, H, D), (stride, H * D, D, 1)).copy_(a[n].to(DEV)).requires_grad_(True)
+  out, s = F.decay_attention(far['q'], far['k'], far['v'], a['decay'].to(DEV), start=a['start'].to(DEV),
+                             state=a['state'].to(DEV))
+  gr = torch.autograd.grad([out, s], [far[n] for n in ('q', 'k', 'v')], [a['gy'].to(DEV), a['gstate'].to(DEV)])
+  for n, t in zip(('out', 'state', 'dq', 'dk', 'dv'), (out, s) + gr):
+    assert torch.equal(base[n], t), n
+
+
+def test_decay_attention_on_one_thread_and_with_a_state_written_since():
+  """The engine's single-threaded mode; a step that writes a saved state in place is noticed."""
+  a = _inputs(40, 2, 2, 16, 16)
+  base = _run(a)
+  with torch.autograd.set_multithreading_enabled(False):
+    got = _run(a)
+  for n in base:
+    assert torch.equal(base[n], got[n]), n
+  dev = {n: (t.to(DEV) if t is not None else None) for n, t in a.items()}
+  q = dev['q'].requires_grad_(True)
+  out, _ = F.decay_attention(q, dev['k'], dev['v'], dev['decay'], state=dev['state'])
+  with torch.no_grad():
+    F.decay_attention_step(q[0], dev['k'][0], dev['v'][0], dev['decay'], dev['state'], out_state=dev['state'])
+  with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+    out.sum().backward()

@@ -82,14 +82,15 @@ class SkinnyLinear(nn.Linear):
 
 
 class LayerNorm(nn.LayerNorm):
-  """nn.LayerNorm over the last dimension (same parameters, same values) on the HIP layer (csrc/trl_norm.hip) for device
-  batches; `relu=True` applies the ReLU behind it in the same launch.  CPU tensors and config.fused_mlp = False take torch's."""
+  """nn.LayerNorm over the last dimension (same parameters, same values) on the HIP layer (csrc/trl_norm.hip) for float32,
+  bfloat16 and float16 device batches; `relu=True` applies the ReLU behind it in the same launch.  Anything else, and
+  config.fused_mlp = False, takes torch's."""
 
   def __init__(self, width, eps=1e-5):
     super().__init__(int(width), eps=eps)
 
   def forward(self, x, relu=False):
-    if x.is_cuda and _fused_mlp_enabled():
+    if x.is_cuda and x.dtype in _F.LAYER_DTYPES and _fused_mlp_enabled():
       return _F.layer_norm(x, self.weight, self.bias, self.eps, relu=relu)
     x = super().forward(x)
     return torch.relu(x) if relu else x
@@ -107,8 +108,16 @@ class Dropout(nn.Module):
     if not 0.0 <= p < 1.0:
       raise ValueError('Dropout: p must be in [0, 1), got %r' % (p,))
     self.p = float(p)
+    self._given = seed
     self._rng = _F.ActRng(seed)
     self.register_buffer('calls', torch.zeros(1, dtype=torch.int64))
+
+  def __deepcopy__(self, memo):
+    """A copy (a target network's layer) draws masks of its own, unless the seed was given."""
+    twin = memo[id(self)] = Dropout(self.p, self._given)
+    twin.calls = self.calls.clone()
+    twin.training = self.training
+    return twin
 
   def forward(self, x, residual=None):
     if not self.training or self.p == 0.0:

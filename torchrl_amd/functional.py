@@ -569,16 +569,14 @@ def linear_u8(x, weight, bias, relu=False):
 
 
 # ------------------------------------------------------------------------------ layer norm, dropout
-_LAYER_DTYPES = {torch.float32: _lib.TRL_F32, torch.bfloat16: _lib.TRL_BF16, torch.float16: _lib.TRL_F16}
+LAYER_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _layer_dtype(t, what):
-  """C element type of a device tensor of the layer kernels (float32, bfloat16, float16)."""
+  """A device tensor of one of the layer kernels' element types."""
   _lib.require_device(t, what)
-  code = _LAYER_DTYPES.get(t.dtype)
-  if code is None:
+  if t.dtype not in LAYER_DTYPES:
     raise TypeError('%s must be float32, bfloat16 or float16, got %s' % (what, t.dtype))
-  return code
 
 
 def _beside(t, other, what):
@@ -663,7 +661,7 @@ _MAX_HEAD = 128
 
 def _decay_operands(fn, q, k, v, decay, lead):
   """Checks what the sequence and the single-step form share; lead: dimensions in front of [H, D]."""
-  code = _layer_dtype(q, fn + ': q')
+  _layer_dtype(q, fn + ': q')
   for t, what in ((k, 'k'), (v, 'v')):
     _beside(t, q, '%s: %s' % (fn, what))
     if t.dtype != q.dtype:
@@ -680,7 +678,6 @@ def _decay_operands(fn, q, k, v, decay, lead):
     raise ValueError('%s: decay must be float32 [%d], got %s %s' % (fn, H, decay.dtype, tuple(decay.shape)))
   if decay.requires_grad:
     raise ValueError('%s: decay is a constant of the layer and gets no gradient' % fn)
-  return code
 
 
 def _start_flags(fn, start, q, shape):
@@ -741,7 +738,7 @@ def decay_attention_step(q, k, v, decay, state, scale=None, start=None, out_stat
   [N, H, Dv], the new state), one launch.  out_state: where the new state goes (may be `state` itself), a new tensor
   by default.  For acting: it carries no gradients and refuses inputs that ask for them."""
   fn = 'decay_attention_step'
-  code = _decay_operands(fn, q, k, v, decay, 1)
+  _decay_operands(fn, q, k, v, decay, 1)
   N, H, dk = q.shape
   dv = v.shape[2]
   start, start_code = _start_flags(fn, start, q, (N,))
