@@ -452,17 +452,36 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
       fetch(q, begin);
       continue;
     }
-    const int m = one < 0 ? chunk : 1;
-    cut |= F != 0;
-    if constexpr (OUT) {
-      f32x4 p;
-      if (F == 0) {
+    if (chunk == 16 && one < 0 && F == 0) {
+      // the usual chunk, whole and of one episode: no branch in it (the loop of a few workgroups is a chain of instructions,
+      // some 4,300 cycles a chunk with a branch at every place where chunks differ)
+      if constexpr (OUT) {
+        f32x4 p;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           p[r] = 4 * g + r <= x ? P[r] * w_intra[r] : 0.f;
           o[r] *= w_inter[r];
         }
-      } else {
+        o = M::mma_left(M::split(p), C, o);
+        if (col < dc) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) po[r * out_step] = (T)o[r];
+        }
+        po += 16 * out_step;
+      }
+      const typename M::Weighed wc = M::weigh(C, w_state);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        // (lambda^16 in two parts: its rounding would otherwise repeat in the same direction every chunk)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[kt][r] = fmaf(S[kt][r], full_hi, S[kt][r] * full_lo);
+        S[kt] = M::mma_state(*(const V4 *)(BT + col_at(kt * 16 + x, 4 * g)), wc, S[kt]);
+      }
+    } else {
+      const int m = one < 0 ? chunk : 1;
+      cut |= F != 0;
+      if constexpr (OUT) {
+        f32x4 p;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int j = 4 * g + r;
@@ -471,56 +490,38 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
           p[r] = on ? P[r] * w_intra[r] : 0.f;
           o[r] = (F & le_j) == 0 ? o[r] * w_inter[r] : 0.f;
         }
-      }
-      o = M::mma_left(M::split(p), C, o);
-if (m == 16 && dc == 16 * waves) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) po[r * out_step] = (T)o[r];
-      } else {
+        o = M::mma_left(M::split(p), C, o);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if ((4 * g + r < m) & (col < dc)) po[r * out_step] = (T)o[r];
+        po += m * out_step;
       }
-      po += m * out_step;
-    }
-    float hi = full_hi, lo = full_lo, ws[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) ws[e] = w_state[e];
-    if (m != 16) {
-      hi = pw[16 + m], lo = pw_lo[m];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) ws[e] = pw[16 + m - off - 4 * g - e] * s.s_state;
-    }
-    if (F != 0) {
       // steps that a start keeps from the chunk's end weigh nothing (b and c are finite, or this is one step alone)
+      float ws[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ws[e] = (F & ~((1u << (4 * g + e + off)) - 1)) == 0 ? ws[e] : 0.f;
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) S[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    } else {
-      // (lambda^m in two parts: its rounding would otherwise repeat in the same direction every chunk)
+      for (int e = 0; e < 4; ++e)
+        ws[e] = (F & ~((1u << (4 * g + e + off)) - 1)) == 0 ? pw[16 + m - off - 4 * g - e] * s.s_state : 0.f;
+      const float hi = pw[16 + m], lo = pw_lo[m];
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) S[kt][r] = fmaf(S[kt][r], hi, S[kt][r] * lo);
-    }
-    // (one step alone whose own start cuts it off -- backward in time -- leaves nothing, whatever c holds)
-    if (!any_bad || off == 1 || F == 0) {
-      const typename M::Weighed wc = M::weigh(C, ws);
+        for (int r = 0; r < 4; ++r) S[kt][r] = F == 0 ? fmaf(S[kt][r], hi, S[kt][r] * lo) : 0.f;
+      // (one step alone whose own start cuts it off -- backward in time -- leaves nothing, whatever c holds)
+      if (!any_bad || off == 1 || F == 0) {
+        const typename M::Weighed wc = M::weigh(C, ws);
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const V4 bt = *(const V4 *)(BT + col_at(kt * 16 + x, 4 * g));
-        S[kt] = M::mma_state(bt, wc, S[kt]);
+        for (int kt = 0; kt < KT; ++kt)
+          S[kt] = M::mma_state(*(const V4 *)(BT + col_at(kt * 16 + x, 4 * g)), wc, S[kt]);
       }
-    }
-    if (any_bad) {             // rows past da: 0 times a value that is not finite
-      int rows = da - 4 * g;
-      asm volatile("" : "+v"(rows));      // (its comparisons are made here, not kept over the loop)
+      if (any_bad) {           // rows past da: 0 times a value that is not finite
+        int rows = da - 4 * g;
+        asm volatile("" : "+v"(rows));      // (its comparisons are made here, not kept over the loop)
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (kt * 16 + r >= rows) S[kt][r] = 0.f;
+          for (int r = 0; r < 4; ++r)
+            if (kt * 16 + r >= rows) S[kt][r] = 0.f;
+      }
     }
     if (one < 0 || ++one == chunk) {
       begin += chunk;
