@@ -233,8 +233,10 @@ constexpr int lds_bytes(int waves) {
 // A workgroup carries one (env, head, segment) of one of the scans (blockIdx.y) through time, a wave 16 of c's columns (waves
 // past them only help to stage).  KT: 16-column tiles of a's (b's) dimension, at most the workgroup's waves: every thread brings
 // one quad of a, of b and of c.  VEC: both dimensions are multiples of four.
+// Registers for four waves a SIMD; with 8 tiles (a workgroup of 8 waves) for two, one workgroup a CU: at 128 registers S and its
+// operands spill (128 steps of 2,048 heads of 128, training: f32 1,310 -> 1,025 us, bf16 837 -> 676).
 template <typename T, int KT, bool OUT, bool VEC>
-__global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
+__global__ __launch_bounds__(512, KT == 8 ? 2 : 4) void k_scan(Scans all) {
   typedef typename Quad<T>::M M;
   typedef typename Quad<T>::Lds V4;
   typedef typename Quad<T>::L L;
@@ -270,7 +272,7 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
   const int64_t sa = dir * s.a.st, sb = dir * s.b.st, sc = dir * s.c.st;
 
   // Every quad of a whole chunk is inside its operand: nothing to select when it is staged.  Where that is worth code of its own:
-  // bf16 with the usual sizes (256 steps of 256 heads of 64: 80 -> 74 us; f32 loses 4% to the longer loop).
+  // bf16 with the usual sizes (256 steps of 256 heads of 64: 72 -> 68 us; f32 loses 4% to the longer loop).
   constexpr bool kWhole = VEC && !M::kShare && (KT & (KT - 1)) == 0;
   const bool whole = kWhole && waves == KT && da == 16 * KT && dc == 16 * KT;
   struct Quads {
@@ -308,9 +310,15 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
       put(q.a.template get<true>(), b, c, arow, crow);
       return (int)M::bad(M::doubt(b)) | (int)M::bad(M::doubt(c));
     }
-    const int na = (one < 0 ? arow < m : arow == one) ? da - acol : 0, nc = (one < 0 ? crow < m : crow == one) ? dc - ccol : 0;
-    const V4 b = quad_of<T, VEC>(q.b, arow < 16 ? na : 0), c = quad_of<T, VEC>(q.c, nc);
-    put(quad_of<T, VEC>(q.a, na), b, c, one < 0 ? arow : (arow - one) & 15, one < 0 ? crow : (crow - one) & 15);
+    if (one < 0) {
+      const int na = arow < m ? da - acol : 0;
+      const V4 b = quad_of<T, VEC>(q.b, na), c = quad_of<T, VEC>(q.c, crow < m ? dc - ccol : 0);
+      put(quad_of<T, VEC>(q.a, na), b, c, arow, crow);
+      return (int)M::bad(M::doubt(b)) | (int)M::bad(M::doubt(c));
+    }
+    const int na = arow == one ? da - acol : 0;
+    const V4 b = quad_of<T, VEC>(q.b, na), c = quad_of<T, VEC>(q.c, crow == one ? dc - ccol : 0);
+    put(quad_of<T, VEC>(q.a, na), b, c, (arow - one) & 15, (crow - one) & 15);
     return (int)M::bad(M::doubt(b)) | (int)M::bad(M::doubt(c));
   };
 
@@ -408,8 +416,7 @@ __global__ __launch_bounds__(512, 4) void k_scan(Scans all) {
   for (int begin = 0, one = -1; begin < steps; buf ^= 1) {
     const int chunk = std::min(16, steps - begin);
     const bool bad = __any(stage(q, buf, chunk, one) != 0);
-    uint32_t F = 0;          // bit i: step i of the chunk is a start
-    if (s.start != nullptr) F = (uint32_t)__ballot((q.flag != 0.f) & (lane < chunk));
+    uint32_t F = (uint32_t)__ballot((q.flag != 0.f) & (lane < chunk));      // bit i: step i of the chunk is a start
     if (one >= 0) F = (F >> one) & 1;
     if (lane == 0) bad_flag[buf][wave] = bad;
     // the other buffer is written only after every wave has passed this barrier
