@@ -161,3 +161,13 @@ def test_reference_generator_is_the_published_one():
   words = ref.philox_words(9, seed, call)
   for g in range(2):
     assert [int(w) for w in words[4 * g:4 * g + 4]] == rounds([0x87654321, 0x0fedcba9, g, 0x80000000], [0x9abcdef0, 0x12345678])
+
+
+def test_memory_block_from_the_meta_device():
+  import torch
+  from torchrl_amd.contrib.models import MemoryBlock
+  m = MemoryBlock(32, heads=4, head_size=16)
+  values = {k: v.clone() for k, v in m.state_dict().items()}
+  m = m.to('meta').to_empty(device='cpu')
+  m.load_state_dict(values)
+  assert m.decay.dtype == torch.float32 and torch.equal(m.decay, values['decay'])

@@ -1,7 +1,7 @@
 """Policy / value networks of the four controllers (reference: torchrl/contrib/models.py).
 
-These stay plain torch.nn modules: their matmuls run on PyTorch-ROCm (hipBLASLt / MFMA),
-the one place of the learner where matrix cores are used.  What has to hold for drop-in
+These stay plain torch.nn modules with the reference's parameters; on the device their stacks run on the framework's own
+kernels where those win (config.fused_mlp), else on torch's.  What has to hold for drop-in
 parity is (1) the parameter names, so a reference state_dict loads, (2) the order in which
 parameters are created and re-initialised, so that under the same torch seed the weights
 are bit-identical to the reference's, and (3) the forward arithmetic.  Hidden sizes are
@@ -101,7 +101,8 @@ class Dropout(nn.Module):
   element) and are never stored (csrc/trl_norm.hip).  The call number is a device buffer that every training call draws
   from and raises on the stream, so a step captured into a HIP graph gets a new mask at every replay, and a checkpoint
   carries on where it was taken.  seed: by default torch.initial_seed() mixed with a number that differs for every layer of
-  the process and every rank.  In eval mode x passes through."""
+  the process and every rank.  In eval mode x passes through.  A forward pass that is run again for its gradients (activation
+  checkpointing) would draw another mask: give functional.dropout the call number there."""
 
   def __init__(self, p, seed=None):
     super().__init__()
@@ -439,7 +440,8 @@ class MemoryBlock(nn.Module):
     """Casts of the module leave the decays in float32 (1 - 2^-10 is 1 in bfloat16)."""
     decay = self.decay
     super()._apply(fn, recurse)
-    self.decay = decay.to(self.decay.device)
+    if not decay.is_meta:      # (from there only to_empty: the values come with a state dict)
+      self.decay = decay.to(self.decay.device)
     return self
 
   def _heads(self, x):
