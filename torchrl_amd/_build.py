@@ -1,4 +1,5 @@
-"""Build libtrl_hip.so in-tree with hipcc for gfx950 (cross-compiles without a GPU).
+"""Build libtrl_hip.so in-tree with hipcc for gfx950 (cross-compiles without a GPU), and beside it trl_autograd.so, the layer
+functions' graph nodes (host code, g++).
 
     python -m torchrl_amd._build            # rebuild if sources are newer than the library
     python -m torchrl_amd._build --force

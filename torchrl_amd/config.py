@@ -16,7 +16,8 @@ library computes.
                    split exactly into three bf16 parts and six of the nine partial products kept (f32 accumulators): the
                    accuracy class of an f32 dot product, not the same bits (csrc/trl_learn.hip, k_ac_learn_pair_bx).  A
                    controller's own `products=` argument overrides it.
-  fused_mlp        Linear(+ReLU) stacks use the MFMA layer kernels (csrc/trl_mlp.hip) where they win; False: torch's.
+  fused_mlp        Linear(+ReLU) stacks use the MFMA layer kernels (csrc/trl_mlp.hip) where they win, and LayerNorm modules
+                   the layer norm kernels (csrc/trl_norm.hip); False: torch's.
   force_gradsync   keep the gradient all-reduce in the step at world size 1 (rehearses the N-rank call sequence on one GPU).
   async_allreduce  None: stream-ordered collective with RCCL, blocking with gloo; True / False forces either.
   kernel_push      small host pushes go through the push kernel reading pinned records (False: async H2D copies).

@@ -13,14 +13,17 @@
 // dk: (v, do, q) and dv: (k, q, do) backward in time -- so ONE kernel computes the output and the three gradients.  Its
 // operands are called a (the q role), b (the k role) and c (the v role) below.
 //
-// One wave carries one (env, head, group of c's columns) through time with S in MFMA accumulators: 16 steps a turn, all
-// products on the exact-f32 16x16x4 MFMA.  Every accumulator is used where it lies: lane (g = lane / 16, x = lane % 16) of a
-// result tile holds rows 4g .. 4g + 3 of column x, which is just what the same instruction takes as an operand with k = 4g + e
-// (the sum over k may run in any order as long as both operands agree).  So the pair products are made transposed
-// (P^T = b a^T: the next product's left operand) and S multiplies from the right, with no exchange between lanes and no LDS.
+// One workgroup carries one (env, head, time segment), each of its waves 16 of c's columns, with the wave's columns of S in MFMA
+// accumulators from the first step to the last: 16 steps a turn, products on the 16x16 MFMA (f32 and f16 inputs: exact f32;
+// bf16 inputs: bf16, where a computed operand goes in as two or three bf16 parts).  Every accumulator is used where it lies:
+// lane (g = lane / 16, x = lane % 16) of a result tile holds rows 4g .. 4g + 3 of column x, which is just what the same
+// instruction takes as an operand with k = 4g + e (the sum over k may run in any order as long as both operands agree).  So the
+// pair products are made transposed (P^T = b a^T: the next product's left operand) and S multiplies from the right, with no
+// exchange between lanes.  The inputs come through LDS, staged a chunk ahead in two buffers: a by rows, b and c transposed.
 //
-// Few rows: time is cut into segments.  A first launch makes every segment's own contribution to the state, a second joins
-// them in order (state entering segment s + 1 = lambda^len state entering s + contribution), a third runs the segments.
+// Few heads: time is cut into segments.  A first launch makes every segment's own contribution to the state, the last runs the
+// segments; the state that enters one (state entering segment s + 1 = lambda^len state entering s + contribution, in order) is
+// made by its workgroup itself, or, with many segments, by a launch between the two.
 //
 // Values that are not finite stay where the recurrence puts them: masks are selections, never products with zero -- except
 // of b's and c's steps inside a chunk, so a chunk whose b or c holds an infinity or a NaN is taken one step at a time.
@@ -50,7 +53,9 @@ __device__ __forceinline__ void load4(const T *row, int col, int dim, bool live,
 }
 
 // seg_state[s]: contribution of segment s -> state entering segment s, in the scan's direction.  coef < 0: a start in it.
-// blockIdx.y: one of the scans.
+// blockIdx.y: one of the scans.  A thread per element of the state, a chain of dependent sums over the segments whose operands
+// are loaded sixteen at a time (64 segments of 8 heads of 64 x 64: 9.6 us; with one load in flight the chain was memory latency
+// alone).
 __global__ __launch_bounds__(kThreads) void k_join(Scans all, int64_t heads, int64_t size) {
   const Scan &s = all.s[blockIdx.y];
   const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -78,7 +83,9 @@ __global__ __launch_bounds__(kThreads) void k_join(Scans all, int64_t heads, int
   }
 }
 
-// one step: a workgroup per (env, head); LC lanes hold four columns each, the others share out the rows
+// One step: a workgroup per (env, head); LC lanes hold four columns each (the fewest that hold a row, so that a wave's access
+// is whole rows), the others share out the rows.  Bound by the state's one read and one write: 4,096 envs of 4 heads of 64 x 64
+// take 105 us, 5.1 TB/s; one env 3.5 us.
 template <typename T, int LC>
 __global__ __launch_bounds__(kThreads) void k_step(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
                                                    const float *__restrict__ decay, const void *__restrict__ start,
@@ -122,7 +129,11 @@ __global__ __launch_bounds__(kThreads) void k_step(const T *__restrict__ q, cons
   }
 }
 
-// time segments: enough workgroups to fill the chip, of at least 64 steps each
+// Time segments: as many as bring the launch to 512 workgroups (two a CU), each of at least 64 steps -- and none where that makes
+// fewer than three, since a contribution costs most of a segment's work again, so that two halves take as long as the whole.
+// Training passes in f32, heads of 64, with and without: 256 heads of 256 steps, two segments 128 us, one 105; 128 heads of 128
+// steps, two 43.7, one 41; 128 heads of 1,024 steps, four 219, one 296.  8 heads of 8,192 steps in bf16: 64 segments (512
+// workgroups) 137 us, 32 segments 151, 128 segments 158.
 void segments(int64_t T, int64_t heads, int *segs, int *seg_len) {
   int64_t want = heads > 0 ? trl_cdiv(512, heads) : 1;
   want = std::max<int64_t>(1, std::min<int64_t>(want, T / 64));

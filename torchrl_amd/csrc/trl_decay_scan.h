@@ -219,7 +219,8 @@ __device__ __forceinline__ int col_at(int col, int row) {
 // (kShare) or b by rows too.
 // Every wave needs all pair products.  In f32 they would be a third of its matrix instructions (16 of 52 a chunk at 64
 // columns), so each wave makes the part of one tile of columns and the parts are added through LDS, behind a second barrier:
-// 677 -> 592 us for a training pass over 256 steps of 2,048 heads.  On the bf16 MFMA all of them cost 4 instructions of half
+// 677 -> 592 us for a training pass over 256 steps of 2,048 heads.  (Closing a chunk's output behind the next chunk's first
+// barrier instead, which saves the second: 528 -> 558 us, the values carried over spill.)  On the bf16 MFMA all of them cost 4 instructions of half
 // the length, less than the exchange takes.
 template <typename T, int KT, bool OUT>
 __host__ __device__ constexpr int chunk_elems(int waves) {
@@ -234,9 +235,11 @@ constexpr int lds_bytes(int waves) {
 // past them only help to stage).  KT: 16-column tiles of a's (b's) dimension, at most the workgroup's waves: every thread brings
 // one quad of a, of b and of c.  VEC: both dimensions are multiples of four.
 // Registers for four waves a SIMD; with 8 tiles (a workgroup of 8 waves) for two, one workgroup a CU: at 128 registers S and its
-// operands spill (128 steps of 2,048 heads of 128, training: f32 1,310 -> 1,025 us, bf16 837 -> 676).
+// operands spill (128 steps of 2,048 heads of 128, training: f32 1,310 -> 1,025 us, bf16 837 -> 676).  With 6 tiles in f32 for
+// three (heads of 96: 876 -> 808 us; bf16, which spills less, loses there: 507 -> 610), with 5 tiles four are best (heads of 80:
+// f32 600 us against 733 with three, bf16 412 against 558).
 template <typename T, int KT, bool OUT, bool VEC>
-__global__ __launch_bounds__(512, KT == 8 ? 2 : 4) void k_scan(Scans all) {
+__global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 3 : 4) void k_scan(Scans all) {
   typedef typename Quad<T>::M M;
   typedef typename Quad<T>::Lds V4;
   typedef typename Quad<T>::L L;

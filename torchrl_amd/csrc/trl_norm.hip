@@ -10,6 +10,9 @@
 // The weight's and the bias's gradients need a sum over all rows: every lane owns fixed columns, adds them up over the rows
 // its workgroup walks, the workgroup's lane groups are added in order, and a second launch adds the workgroups' partial sums
 // in order: no atomics, the same bits every run.
+// Measured: 1M x 64 f32 forward 96 us (5.6 TB/s), backward 160 us (5.0 TB/s) + 5 us for the join of the parts; 16k x 1024 bf16
+// 13.0, 21.8 and 4.5 us (the data stay in the last-level cache); 10007 x 257 f32 8.8, 10.0 and 4.2; 16 x 64 1.6 us.  A training
+// call on small data is bound by the host and the graph engine (46 us and more), not by these.
 #include <algorithm>
 
 #include "trl_io.h"
@@ -246,7 +249,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd(const T *__restrict__ gy,
     }
 }
 
-// rows wider than the registers of a workgroup: one workgroup a row, the row read once per pass (from L2 after the first)
+// Rows wider than the registers of a workgroup (more than 8,192 f32 or 16,384 elements of 16 bits): one workgroup a row, the
+// row read once per pass (from L2 after the first).  Correct at any width; not tuned: no network here is that wide.
 template <typename T, bool ACT>
 __global__ __launch_bounds__(kThreads) void k_norm_fwd_wide(const T *__restrict__ x, const float *__restrict__ w,
                                                             const float *__restrict__ b, int64_t rows, int64_t width,
@@ -361,7 +365,10 @@ __global__ __launch_bounds__(1024) void k_norm_fold(const float *__restrict__ pa
 }
 
 // Lanes a row and 16 B slots a lane by the number of slots of a row: the fewest lanes that hold it in few slots, so that a
-// wave works on several narrow rows at once; 0 = wider than a workgroup's registers
+// wave works on several narrow rows at once and up to 256 slots need no barrier; 0 = wider than a workgroup's registers.
+// Training passes against a wave for every row of at most 64 slots and a workgroup for wider ones: 1M x 32 f32 134 us against
+// 384, 1M x 64 263 / 423, 256k x 128 bf16 62 / 117, 16k x 512 f32 37 / 47, 64k x 1024 bf16 139 / 233, 10007 x 257 f32 26 / 45;
+// even only for 16k x 1024 f32 (66 / 64).
 struct Shape {
   int lpr, nv;
 };
