@@ -530,3 +530,41 @@ def test_decay_attention_on_one_thread_and_with_a_state_written_since():
     F.decay_attention_step(q[0], dev['k'][0], dev['v'][0], dev['decay'], dev['state'], out_state=dev['state'])
   with pytest.raises(RuntimeError, match='modified by an inplace operation'):
     out.sum().backward()
+
+
+def test_decay_attention_of_one_tensor_in_three_roles():
+  """q, k and v the same tensor: its gradient is the sum of the three."""
+  g = torch.Generator().manual_seed(3)
+  x = torch.randn(200, 3, 2, 24, generator=g).to(DEV).requires_grad_(True)
+  gy = torch.randn(200, 3, 2, 24, generator=g).to(DEV)
+  decay = torch.tensor([0.9, 0.99], device=DEV)
+  one, = torch.autograd.grad(F.decay_attention(x, x, x, decay)[0], [x], gy)
+  three = [x.detach().clone().requires_grad_(True) for _ in range(3)]
+  q, k, v = torch.autograd.grad(F.decay_attention(*three, decay)[0], three, gy)
+  # (two additions in float32, in an order that is the engine's)
+  assert torch.all((one - (q + k + v)).abs() <= 2 * torch.finfo(torch.float32).eps * (q.abs() + k.abs() + v.abs()))
+
+
+def test_memory_block_under_autocast():
+  m = _block(dropout=0.25).train()
+  x = torch.randn(40, 3, 48, device=DEV, requires_grad=True)
+  with torch.autocast('cuda', torch.bfloat16):
+    y, s = m(x)
+    m.eval()
+    z, _ = m(x)
+  assert y.dtype == z.dtype == torch.float32 and s.dtype == torch.float32
+  y.sum().backward()
+  assert torch.isfinite(x.grad).all() and all(torch.isfinite(p.grad).all() for p in m.parameters())
+
+
+def test_decay_attention_in_inference_mode():
+  q = torch.randn(30, 2, 1, 8, device=DEV)
+  decay = torch.full((1,), 0.95, device=DEV)
+  want, last = F.decay_attention(q, q, q, decay)
+  with torch.inference_mode():
+    out, state = F.decay_attention(q, q, q, decay)
+    assert torch.equal(out, want) and torch.equal(state, last)
+    st = torch.zeros(2, 1, 8, 8, device=DEV)
+    for t in range(30):
+      o, st = F.decay_attention_step(q[t], q[t], q[t], decay, st, out_state=st)
+  torch.testing.assert_close(st, last, rtol=1e-5, atol=1e-5)

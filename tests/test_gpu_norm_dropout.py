@@ -454,3 +454,34 @@ def test_layer_norm_module_takes_other_types_through_torch():
   m = LayerNorm(16).to(DEV).double()
   x = torch.randn(4, 16, device=DEV, dtype=torch.float64)
   torch.testing.assert_close(m(x), torch.nn.functional.layer_norm(x, (16,), m.weight, m.bias))
+
+
+def test_one_tensor_in_two_roles():
+  """dropout(x, residual=x) and layer_norm(x, w, w): the gradients of both roles add up."""
+  x = torch.randn(300, 40, generator=_gen(0)).to(DEV).requires_grad_(True)
+  gy = torch.randn(300, 40, generator=_gen(1)).to(DEV)
+  y = F.dropout(x, 0.5, 3, 4, residual=x)
+  keep = F.dropout(torch.ones_like(x), 0.5, 3, 4)      # 0 or 2
+  assert torch.equal(y, x + keep * x)
+  g, = torch.autograd.grad(y, [x], gy)
+  assert torch.equal(g, gy + keep * gy)
+  w = torch.randn(40, generator=_gen(2)).to(DEV).requires_grad_(True)
+  u, v = w.detach().clone().requires_grad_(True), w.detach().clone().requires_grad_(True)
+  one, = torch.autograd.grad(F.layer_norm(x, w, w), [w], gy)
+  two = torch.autograd.grad(F.layer_norm(x, u, v), [u, v], gy)
+  assert torch.equal(one, two[0] + two[1])
+
+
+def test_dropout_module_with_a_residual_of_another_type():
+  """As under autocast: the branch in bfloat16, the residual in float32; training has the type that eval mode has."""
+  from torchrl_amd.contrib.models import Dropout
+  m = Dropout(0.5, seed=5).to(DEV)
+  x = torch.randn(200, 16, generator=_gen(0)).bfloat16().to(DEV).requires_grad_(True)
+  r = torch.randn(200, 16, generator=_gen(1)).to(DEV).requires_grad_(True)
+  y = m(x, residual=r)
+  assert y.dtype == m.eval()(x, residual=r).dtype == torch.float32
+  assert torch.equal(y, F.dropout(x.float(), 0.5, 5, 0, residual=r))
+  gx, gr = torch.autograd.grad(y.sum(), [x, r])
+  assert gx.dtype == torch.bfloat16 and torch.equal(gr, torch.ones_like(r))
+  y = m(r, residual=x)
+  assert y.dtype == torch.float32

@@ -99,8 +99,8 @@ class LayerNorm(nn.LayerNorm):
 class Dropout(nn.Module):
   """Dropout with an optional residual, y = residual + dropout(x), whose masks are functions of (seed, call number,
   element) and are never stored (csrc/trl_norm.hip).  The call number is a device buffer that every training call draws
-  from and raises on the stream, so a step captured into a HIP graph gets a new mask at every replay, and a checkpoint
-  carries on where it was taken.  seed: by default torch.initial_seed() mixed with a number that differs for every layer of
+  from and raises on the stream, so a step captured into a HIP graph gets a new mask at every replay, and under
+  the same seed a checkpoint carries on where it was taken.  seed: by default torch.initial_seed() mixed with a number that differs for every layer of
   the process and every rank.  In eval mode x passes through.  A forward pass that is run again for its gradients (activation
   checkpointing) would draw another mask: give functional.dropout the call number there."""
 
@@ -123,6 +123,9 @@ class Dropout(nn.Module):
   def forward(self, x, residual=None):
     if not self.training or self.p == 0.0:
       return x if residual is None else residual + x
+    if residual is not None and residual.dtype != x.dtype:      # (under autocast; the type that eval mode's sum has)
+      dtype = torch.promote_types(x.dtype, residual.dtype)
+      x, residual = x.to(dtype), residual.to(dtype)
     seed, _ = self._rng.next()
     return _F.dropout(x, self.p, seed, _F.next_call(self.calls), residual=residual)
 
