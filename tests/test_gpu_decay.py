@@ -568,3 +568,40 @@ def test_decay_attention_in_inference_mode():
     for t in range(30):
       o, st = F.decay_attention_step(q[t], q[t], q[t], decay, st, out_state=st)
   torch.testing.assert_close(st, last, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('dk,dv', [(16, 16), (33, 40), (64, 64), (128, 100)])
+def test_decay_attention_flags_of_long_sequences(dk, dv, dtype):
+  """Enough heads that time is not cut and more steps than a workgroup takes flags of at once; some envs against the reference,
+  uint8 flags bit for bit against float32 ones."""
+  a = _inputs(530, 257, 1, dk, dv, dtype=dtype, cuts=0.02, ragged=True, decay=[0.97])
+  a['lengths'][:3] = torch.tensor([530, 529, 513], dtype=torch.int32)
+  a['start'][[0, 63, 64, 128, 192, 255, 256, 512, 529]] = 1.0
+  a['start'][:, 1] *= -0.0      # (-0 is no start)
+  got = _run(a)
+  some = [0, 1, 2, 100, 256]
+  part = {n: t if n == 'decay' else t[some] if n in ('lengths', 'state', 'gstate') else t[:, some] for n, t in a.items()}
+  kw = {n: part[n] for n in ('start', 'lengths', 'state', 'gy', 'gstate')}
+  want = ref.decay_attention(part['q'], part['k'], part['v'], part['decay'], **kw)
+  bound = ref.decay_bounds(part['q'], part['k'], part['v'], part['decay'], dtype, **kw)
+  for n, t in got.items():
+    ref.check(t[some] if n in ('state', 'dstate') else t[:, some], want[n], bound[n], n)
+  b = _run(dict(a, start=(a['start'] != 0).to(torch.uint8)))
+  assert all(torch.equal(got[n], b[n]) for n in got)
+
+
+def test_decay_attention_a_not_finite_step_between_flags():
+  """An infinity in the first step of a block of flags, a start behind it: nothing of it after the start."""
+  a = _inputs(200, 257, 1, 16, 16, decay=[0.97])
+  a['start'] = torch.zeros(200, 257)
+  a['start'][[65, 130]] = 1.0
+  clean = _run(a, grads=False)['out']
+  a['k'][64] = float('inf')
+  out = _run(a, grads=False)['out']
+  assert torch.equal(out[:64], clean[:64]) and not torch.isfinite(out[64]).any()
+  # (its chunk's later steps are taken one by one: the same sums in another order, of up to 65 terms and 16 products each)
+  terms = 4 * (65 + 16) * torch.finfo(torch.float32).eps
+  size = ref.decay_attention(a['q'].abs()[65:], _inputs(200, 257, 1, 16, 16, decay=[0.97])['k'].abs()[65:], a['v'].abs()[65:],
+                             a['decay'], start=a['start'][65:])['out']
+  assert torch.all((out[65:] - clean[65:]).abs().double().cpu() <= terms * size)

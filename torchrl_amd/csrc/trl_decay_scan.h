@@ -88,9 +88,13 @@ struct Math32 {
     return f32x4{c[0] * w[0], c[1] * w[1], c[2] * w[2], c[3] * w[3]};
   }
   static __device__ __forceinline__ f32x4 mma_state(const In &b, const In &wc, f32x4 s) { return mma(b, wc, s); }
-  // not zero where a value is not finite (0 times it is a NaN)
-  static __device__ __forceinline__ float doubt(const In &v) { return v[0] * 0.f + v[1] * 0.f + (v[2] * 0.f + v[3] * 0.f); }
-  static __device__ __forceinline__ bool bad(float doubt) { return doubt != 0.f; }
+  // whether a value is not finite (0 times it is a NaN)
+  static __device__ __forceinline__ bool bad(const In &u, const In &v) {
+    float d = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d = fmaf(u[e], 0.f, fmaf(v[e], 0.f, d));
+    return d != 0.f;
+  }
 };
 
 // bf16: one 16x16x16 product of the inputs as they are; what is computed in f32 goes in as a sum of bf16 parts, two of them
@@ -142,13 +146,13 @@ struct Math16 {
   static __device__ __forceinline__ f32x4 mma_state(const In &b, const Weighed &wc, f32x4 s) {
     return mma(b, wc.hi, mma(b, wc.mid, mma(b, wc.lo, s)));
   }
-  // bit 15 or 31 where an exponent is all ones
+  // whether an exponent is all ones: bit 15 or 31 after the addition
   static __device__ __forceinline__ uint32_t doubt(const In &v) {
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     const u32x2 u = __builtin_bit_cast(u32x2, v);
     return ((u[0] & 0x7F807F80u) + 0x00800080u) | ((u[1] & 0x7F807F80u) + 0x00800080u);
   }
-  static __device__ __forceinline__ bool bad(uint32_t doubt) { return (doubt & 0x80008000u) != 0; }
+  static __device__ __forceinline__ bool bad(const In &u, const In &v) { return ((doubt(u) | doubt(v)) & 0x80008000u) != 0; }
 };
 
 // ---- four consecutive elements of one step as they are loaded (`raw`: nothing touches them before their chunk's turn, so the
@@ -246,6 +250,7 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   constexpr int ROW = 16 * KT + 4;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   __shared__ int bad_flag[2][8];
+  __shared__ uint64_t marks[2][8];
   __shared__ float pw[48], pw_lo[32];
   const Scan &s = all.s[blockIdx.y];
   const int tid = threadIdx.x, waves = blockDim.x >> 6;
@@ -280,53 +285,50 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   const bool whole = kWhole && waves == KT && da == 16 * KT && dc == 16 * KT;
   struct Quads {
     Quad<T> a, b, c;
-    float flag;                // of step x
   };
-  auto fetch = [&](Quads &q, int at) {      // the chunk that begins with step `at` (none past the end)
-    const int m = steps - at;
+  auto fetch = [&](Quads &q, int at, int cap) {      // the chunk of up to `cap` steps from `at` on (none past the end)
+    const int m = std::min(cap, steps - at);
     const int na = arow < m ? da - acol : 0, nc = crow < m ? dc - ccol : 0;
     if constexpr (OUT) fetch_quad<T, VEC>(q.a, pa + at * sa, na);
     fetch_quad<T, VEC>(q.b, pb + at * sb, na);
     fetch_quad<T, VEC>(q.c, pc + at * sc, nc);
-    if (s.start != nullptr && x < m) {
-      const int64_t i = (t_first + dir * (at + x)) * s.N + n;
-      q.flag = s.start_u8 ? (float)((const uint8_t *)s.start)[i] : ((const float *)s.start)[i];
+  };
+  // The flags of 64 steps a wave at a time, loaded that many steps ahead; as bits in `marks` once their turn has come.  (Loaded
+  // with every chunk their addresses and conversions cost more than they look: 256 steps of 2,048 heads of 64, training, float32
+  // flags 554 -> 536 us, uint8 flags, whose conversion waited for the chunk's loads, 600 -> 536.)
+  const int marks_len = 64 * waves;
+  uint32_t flag = 0;           // as it was loaded
+  auto fetch_flag = [&](int at) {
+    flag = 0;
+    if (s.start != nullptr && at + tid < steps) {
+      const int64_t i = (t_first + dir * (at + tid)) * s.N + n;
+      flag = s.start_u8 ? ((const uint8_t *)s.start)[i] : ((const uint32_t *)s.start)[i];
     }
   };
   auto lds = [&](int buf) { return (L *)lds_raw + buf * chunk_elems<T, KT, OUT>(waves); };
   f32x4 *const parts = (f32x4 *)((L *)lds_raw + 2 * chunk_elems<T, KT, OUT>(waves));
-  // the chunk's m steps (one < 0), or its step `one` alone as the first of a chunk of its own; whether b or c is not finite
-  auto stage = [&](const Quads &q, int buf, int m, int one) {
+  // the chunk's m steps into a buffer; whether b or c is not finite
+  auto stage = [&](const Quads &q, int buf, int m) {
     L *A = lds(buf), *B = A + 16 * ROW, *BT = A + (OUT ? (M::kShare ? 1 : 2) * 16 * ROW : 0), *CC = BT + 16 * KT * kColStride;
-    auto put = [&](V4 a, V4 b, V4 c, int ra, int rc) {
+    auto put = [&](V4 a, V4 b, V4 c) {
       if (KT >= 8 || arow < 16) {
-        if constexpr (OUT) *(V4 *)(A + ra * ROW + acol) = a;
-        if constexpr (OUT && !M::kShare) *(V4 *)(B + ra * ROW + acol) = b;
+        if constexpr (OUT) *(V4 *)(A + arow * ROW + acol) = a;
+        if constexpr (OUT && !M::kShare) *(V4 *)(B + arow * ROW + acol) = b;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) BT[col_at(acol, ra) + e * kColStride] = b[e];
+        for (int e = 0; e < 4; ++e) BT[col_at(acol, arow) + e * kColStride] = b[e];
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) CC[col_at(ccol, rc) + e * kColStride] = c[e];
+      for (int e = 0; e < 4; ++e) CC[col_at(ccol, crow) + e * kColStride] = c[e];
+      return M::bad(b, c);
     };
-    if (kWhole && whole && m == 16 && one < 0) {
-      const V4 b = q.b.template get<true>(), c = q.c.template get<true>();
-      put(q.a.template get<true>(), b, c, arow, crow);
-      return (int)M::bad(M::doubt(b)) | (int)M::bad(M::doubt(c));
-    }
-    if (one < 0) {
-      const int na = arow < m ? da - acol : 0;
-      const V4 b = quad_of<T, VEC>(q.b, na), c = quad_of<T, VEC>(q.c, crow < m ? dc - ccol : 0);
-      put(quad_of<T, VEC>(q.a, na), b, c, arow, crow);
-      return (int)M::bad(M::doubt(b)) | (int)M::bad(M::doubt(c));
-    }
-    const int na = arow == one ? da - acol : 0;
-    const V4 b = quad_of<T, VEC>(q.b, na), c = quad_of<T, VEC>(q.c, crow == one ? dc - ccol : 0);
-    put(quad_of<T, VEC>(q.a, na), b, c, (arow - one) & 15, (crow - one) & 15);
-    return (int)M::bad(M::doubt(b)) | (int)M::bad(M::doubt(c));
+    if (kWhole && whole && m == 16) return put(q.a.template get<true>(), q.b.template get<true>(), q.c.template get<true>());
+    const int na = arow < m ? da - acol : 0, nc = crow < m ? dc - ccol : 0;
+    return put(quad_of<T, VEC>(q.a, na), quad_of<T, VEC>(q.b, na), quad_of<T, VEC>(q.c, nc));
   };
 
   Quads q = {};
-  fetch(q, 0);
+  fetch(q, 0, 16);
+  fetch_flag(0);
 
   const int col = wave * 16 + x;      // this lane's column of c, of S and of the output
   f32x4 S[KT];
@@ -415,17 +417,26 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   T *po = OUT ? (T *)s.out + ((t_first + dir * 4 * g) * heads + nh) * dc + col : nullptr;      // step 4 g of the chunk
   bool cut = false;            // a start inside this segment
   int buf = 0;
+  int marks_at = -marks_len, marks_buf = 0;      // first step of those in `marks`
+  // cap: 16 steps a chunk, or one up to step `until`
 #pragma unroll 1
-  for (int begin = 0, one = -1; begin < steps; buf ^= 1) {
-    const int chunk = std::min(16, steps - begin);
-    const bool bad = __any(stage(q, buf, chunk, one) != 0);
-    uint32_t F = (uint32_t)__ballot((q.flag != 0.f) & (lane < chunk));      // bit i: step i of the chunk is a start
-    if (one >= 0) F = (F >> one) & 1;
+  for (int begin = 0, cap = 16, until = 0; begin < steps; buf ^= 1) {
+    const int chunk = std::min(cap, steps - begin);
+    const bool bad = __any(stage(q, buf, chunk));
     if (lane == 0) bad_flag[buf][wave] = bad;
-    // the other buffer is written only after every wave has passed this barrier
+    if (begin == marks_at + marks_len) {
+      marks_at = begin;
+      marks_buf ^= 1;
+      const uint64_t bits = __ballot((s.start_u8 ? flag : flag << 1) != 0);      // (-0 is 0)
+      if (lane == 0) marks[marks_buf][wave] = bits;
+      fetch_flag(begin + marks_len);
+    }
+    // the other buffers are written only after every wave has passed this barrier
     __syncthreads();
     const int bad_any = bad_flag[buf][std::min(lane, waves - 1)];
-    if (one < 0 || one == chunk - 1) fetch(q, begin + 16);      // on its way while this chunk is worked on
+    const int mark = ((const uint16_t *)marks[marks_buf])[(begin - marks_at) >> 4];
+    const int next_cap = begin + chunk < until ? 1 : 16;
+    fetch(q, begin + chunk, next_cap);      // on its way while this chunk is worked on
     const L *A = lds(buf), *B = A + 16 * ROW, *BT = A + (OUT ? (M::kShare ? 1 : 2) * 16 * ROW : 0),
             *CC = BT + 16 * KT * kColStride;
     const V4 C = *(const V4 *)(CC + col_at(col, 4 * g));
@@ -456,13 +467,16 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
       }
     }
     const bool any_bad = __any(bad_any);
-    if (any_bad && chunk > 1 && one < 0) {
+    if (any_bad && chunk > 1) {
       // b or c holds an infinity or a NaN, which a weight of zero would spread over the chunk: its steps one at a time
-      one = 0;
-      fetch(q, begin);
+      cap = 1;
+      until = begin + chunk;
+      fetch(q, begin, 1);
       continue;
     }
-    if (chunk == 16 && one < 0 && F == 0) {
+    // bit i: step i of the chunk is a start
+    const uint32_t F = ((uint32_t)__builtin_amdgcn_readfirstlane(mark) >> (begin & 15)) & ((1u << chunk) - 1);
+    if (chunk == 16 && F == 0) {
       // the usual chunk, whole and of one episode: no branch in it (the loop of a few workgroups is a chain of instructions,
       // some 4,300 cycles a chunk with a branch at every place where chunks differ)
       if constexpr (OUT) {
@@ -488,7 +502,7 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
         S[kt] = M::mma_state(*(const V4 *)(BT + col_at(kt * 16 + x, 4 * g)), wc, S[kt]);
       }
     } else {
-      const int m = one < 0 ? chunk : 1;
+      const int m = chunk;
       cut |= F != 0;
       if constexpr (OUT) {
         f32x4 p;
@@ -533,10 +547,8 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
             if (kt * 16 + r >= rows) S[kt][r] = 0.f;
       }
     }
-    if (one < 0 || ++one == chunk) {
-      begin += chunk;
-      one = -1;
-    }
+    begin += chunk;
+    cap = next_cap;
   }
 
   // the state left behind: the caller's at the end of time, or this segment's contribution
