@@ -223,9 +223,9 @@ __device__ __forceinline__ int col_at(int col, int row) {
 // (kShare) or b by rows too.
 // Every wave needs all pair products.  In f32 they would be a third of its matrix instructions (16 of 52 a chunk at 64
 // columns), so each wave makes the part of one tile of columns and the parts are added through LDS, behind a second barrier:
-// 677 -> 592 us for a training pass over 256 steps of 2,048 heads.  (Closing a chunk's output behind the next chunk's first
-// barrier instead, which saves the second: 528 -> 558 us, the values carried over spill.)  On the bf16 MFMA all of them cost 4 instructions of half
-// the length, less than the exchange takes.
+// 677 -> 592 us for a training pass over 256 steps of 2,048 heads (540 with the later steps).  Closing a chunk's output behind
+// the next chunk's first barrier instead, which saves the second, took 632 (the values carried over spill; 567 with registers
+// for three waves a SIMD).  On the bf16 MFMA all pairs cost 4 instructions of half the length, less than the exchange takes.
 template <typename T, int KT, bool OUT>
 __host__ __device__ constexpr int chunk_elems(int waves) {
   return (OUT ? (Quad<T>::M::kShare ? 1 : 2) * 16 * (16 * KT + 4) : 0) + (16 * KT + 16 * waves) * kColStride;
