@@ -605,3 +605,25 @@ def test_decay_attention_a_not_finite_step_between_flags():
   size = ref.decay_attention(a['q'].abs()[65:], _inputs(200, 257, 1, 16, 16, decay=[0.97])['k'].abs()[65:], a['v'].abs()[65:],
                              a['decay'], start=a['start'][65:])['out']
   assert torch.all((out[65:] - clean[65:]).abs().double().cpu() <= terms * size)
+
+
+def test_decay_attention_flags_of_long_sequences_in_one_wave():
+  """As above with workgroups of one wave, whose blocks of flags are 64 steps: heads enough that time is not cut."""
+  for dtype in (torch.float32, torch.bfloat16):
+    a = _inputs(330, 900, 1, 16, 12, dtype=dtype, cuts=0.02, ragged=True, decay=[0.97])
+    a['lengths'][:2] = torch.tensor([330, 321], dtype=torch.int32)
+    a['start'][[0, 63, 64, 128, 192, 255, 256, 320, 329]] = 1.0
+    got = _run(a)
+    some = [0, 1, 100, 899]
+    part = {n: t if n == 'decay' else t[some] if n in ('lengths', 'state', 'gstate') else t[:, some] for n, t in a.items()}
+    kw = {n: part[n] for n in ('start', 'lengths', 'state', 'gy', 'gstate')}
+    want = ref.decay_attention(part['q'], part['k'], part['v'], part['decay'], **kw)
+    bound = ref.decay_bounds(part['q'], part['k'], part['v'], part['decay'], dtype, **kw)
+    for n, t in got.items():
+      ref.check(t[some] if n in ('state', 'dstate') else t[:, some], want[n], bound[n], n)
+
+
+@pytest.mark.parametrize('T,N,H,D', [(4100, 1, 1, 8), (700, 30, 4, 16), (1000, 40, 2, 32), (900, 3, 2, 128)])
+def test_decay_attention_many_segments_of_small_heads(T, N, H, D):
+  """Segments by the number of waves: more than the workgroups join themselves, and as many as they do."""
+  _check(_inputs(T, N, H, D, D, cuts=0.003, ragged=True))

@@ -28,6 +28,7 @@
 // Values that are not finite stay where the recurrence puts them: masks are selections, never products with zero -- except
 // of b's and c's steps inside a chunk, so a chunk whose b or c holds an infinity or a NaN is taken one step at a time.
 #include <algorithm>
+#include <cmath>
 
 #include "trl_decay_scan.h"
 
@@ -129,13 +130,20 @@ __global__ __launch_bounds__(kThreads) void k_step(const T *__restrict__ q, cons
   }
 }
 
-// Time segments: as many as bring the launch to 512 workgroups (two a CU), each of at least 64 steps -- and none where that makes
-// fewer than three, since a contribution costs most of a segment's work again, so that two halves take as long as the whole.
-// Training passes in f32, heads of 64, with and without: 256 heads of 256 steps, two segments 128 us, one 105; 128 heads of 128
-// steps, two 43.7, one 41; 128 heads of 1,024 steps, four 219, one 296.  8 heads of 8,192 steps in bf16: 64 segments (512
-// workgroups) 137 us, 32 segments 151, 128 segments 158.
-void segments(int64_t T, int64_t heads, int *segs, int *seg_len) {
-  int64_t want = heads > 0 ? trl_cdiv(512, heads) : 1;
+// Time segments: as many as bring the launch to 2,048 waves (two a SIMD; a workgroup has one for 16 columns of a head), each of
+// at least 64 steps, no more than sqrt(T) of them, and none where that makes fewer than three.  Training passes, us:
+//  * waves, not workgroups: 128 heads of 128 in bf16, 400 steps: 256 workgroups of 8 waves 178, 512 231; 128 heads of
+//    32 in f32, 400 steps: 768 workgroups of 2 waves 57, 512 65, none 82.
+//  * two halves take as long as the whole, since a contribution costs most of a segment's work again: 256 heads of 64 in f32, 256
+//    steps: two segments 119, one 97; 128 heads, 128 steps: 57 and 49; but 128 heads, 1,024 steps: four 210, one 252.
+//  * shorter ones are mostly start and join, longer ones a longer chain: 64 heads of 64 in bf16, 500 steps: at least 64 steps 72,
+//    128 steps 81; 128 heads of 64, 128 steps: at least 32 steps 61, 64 steps 49.
+//  * the join walks the segments one after another: one head of 16 in f32, 131,072 steps: 362 segments 176, 2,048 485, 128 237;
+//    32,768 steps: 181 segments 95, 512 143.
+void segments(int64_t T, int64_t heads, int32_t dk, int32_t dv, int *segs, int *seg_len) {
+  const int64_t waves = tiles_of(std::max(dk, dv));
+  int64_t want = heads > 0 ? (2048 / waves + heads / 2) / heads : 1;
+  want = std::min(want, (int64_t)std::sqrt((double)T));
   want = std::max<int64_t>(1, std::min<int64_t>(want, T / 64));
   if (want < 3) want = 1;
   const int64_t len = std::max<int64_t>(16, trl_cdiv(trl_cdiv(T, want), 16) * 16);
@@ -187,7 +195,7 @@ extern "C" int64_t trl_decay_attention_workspace_bytes(int64_t T, int64_t N, int
                                                        int32_t backward) {
   if (decay_check("trl_decay_attention_workspace_bytes", T, N, H, dk, dv, TRL_F32)) return TRL_EINVAL;
   int segs, len;
-  segments(T, N * H, &segs, &len);
+  segments(T, N * H, dk, dv, &segs, &len);
   return 4 * seg_floats(N * H, segs, dk, dv) * (backward ? 2 : 1);
 }
 
@@ -221,7 +229,7 @@ extern "C" int trl_decay_attention_fwd(const void *q, const void *k, const void 
   s.dc = dv;
   s.s_inter = s.s_intra = (float)scale;
   s.s_state = 1.f;
-  segments(T, N * H, &s.segs, &s.seg_len);
+  segments(T, N * H, dk, dv, &s.segs, &s.seg_len);
   if (s.segs > 1) {
     TRL_REQUIRE(workspace != nullptr, "%s: null workspace", fn);
     s.seg_state = (float *)workspace;
@@ -257,7 +265,7 @@ extern "C" int trl_decay_attention_bwd(const void *gy, const float *gstate, cons
   s.T = T;
   s.N = N;
   s.H = H;
-  segments(T, N * H, &s.segs, &s.seg_len);
+  segments(T, N * H, dk, dv, &s.segs, &s.seg_len);
   float *ws_s = nullptr, *ws_r = nullptr;
   if (s.segs > 1) {
     TRL_REQUIRE(workspace != nullptr, "%s: null workspace", fn);
