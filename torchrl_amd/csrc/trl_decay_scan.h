@@ -39,7 +39,9 @@ void launch_bf16(const Scans &all, int count, bool out, hipStream_t st);
 void launch_f16(const Scans &all, int count, bool out, hipStream_t st);
 
 // up to so many segments a workgroup joins the contributions before its own by itself: 2 us at 8 of them, against 7 us and a
-// launch for the join of all; beyond, what all workgroups read grows with the square of the segments
+// launch for the join of all; beyond, what all workgroups read grows with the square of the segments.  (Training passes: 64 heads
+// of 64 in bf16, 500 steps in 7 segments: 71 us, joined by the launch 75; 8 heads of 128 in f32, 1,024 steps in 16 segments: by
+// the launch 101, by the workgroups 141.)
 constexpr int kJoinInside = 8;
 
 inline int tiles_of(int dim) { return (dim + 15) / 16; }
