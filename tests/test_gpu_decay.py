@@ -627,3 +627,21 @@ def test_decay_attention_flags_of_long_sequences_in_one_wave():
 def test_decay_attention_many_segments_of_small_heads(T, N, H, D):
   """Segments by the number of waves: more than the workgroups join themselves, and as many as they do."""
   _check(_inputs(T, N, H, D, D, cuts=0.003, ragged=True))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('dk,dv', [(128, 64), (64, 128), (112, 32), (128, 65), (97, 128), (128, 1), (100, 68)])
+def test_decay_attention_wide_heads_in_column_groups(dk, dv, dtype):
+  """Heads of more than 96 are split by columns over workgroups: whole, ragged and missing second groups, with and without
+  segments, and a value that is not finite in one group's columns only."""
+  _check(_inputs(40, 3, 2, dk, dv, dtype=dtype, cuts=0.05, ragged=True))
+  _check(_inputs(260, 1, 2, dk, dv, dtype=dtype, cuts=0.01))
+  a = _inputs(40, 2, 1, dk, dv, dtype=dtype, state=False)
+  clean = _run(a, grads=False)['out']
+  a['v'][20, :, :, dv - 1] = float('inf')
+  out = _run(a, grads=False)['out']
+  assert torch.equal(out[:16], clean[:16]) and not torch.isfinite(out[20:, ..., dv - 1]).any()
+  if dv > 1:      # (the other columns: the same sums, some of them step by step)
+    size = ref.decay_attention(*(torch.nan_to_num(a[n].float(), posinf=0.0).abs() for n in ('q', 'k', 'v')), a['decay'])['out']
+    bound = 8 * (40 + dk) * torch.finfo(torch.float32).eps + torch.finfo(dtype).eps
+    assert torch.all((out - clean)[..., :dv - 1].abs().double().cpu() <= bound * size[..., :dv - 1])

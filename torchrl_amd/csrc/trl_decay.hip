@@ -132,8 +132,8 @@ __global__ __launch_bounds__(kThreads) void k_step(const T *__restrict__ q, cons
 
 // Time segments: as many as bring the launch to 2,048 waves (two a SIMD; a workgroup has one for 16 columns of a head), each of
 // at least 64 steps, no more than sqrt(T) of them, and none where that makes fewer than three.  Training passes, us:
-//  * waves, not workgroups: 128 heads of 128 in bf16, 400 steps: 256 workgroups of 8 waves 178, 512 231; 128 heads of
-//    32 in f32, 400 steps: 768 workgroups of 2 waves 57, 512 65, none 82.
+//  * waves, not workgroups: 128 heads of 128 in bf16, 400 steps: 2,048 waves 178, 4,096 231; 128 heads of 32 in f32, 400
+//    steps: 1,536 waves 57, 1,024 65, 256 82.
 //  * two halves take as long as the whole, since a contribution costs most of a segment's work again: 256 heads of 64 in f32, 256
 //    steps: two segments 119, one 97; 128 heads, 128 steps: 57 and 49; but 128 heads, 1,024 steps: four 210, one 252.
 //  * shorter ones are mostly start and join, longer ones a longer chain: 64 heads of 64 in bf16, 500 steps: at least 64 steps 72,

@@ -237,13 +237,26 @@ constexpr int lds_bytes(int waves) {
   return 2 * chunk_elems<T, KT, OUT>(waves) * (int)sizeof(typename Quad<T>::L) + (OUT && Quad<T>::M::kShare ? KT * 1024 : 0);
 }
 
+// Waves of a workgroup, and quads of a (and b) that each of its threads brings.  With 8 tiles of a's dimension a workgroup of 4
+// waves takes 64 of c's columns (blockIdx.z), so that two of them share a CU and one works while the other starts, ends or waits.
+// Training passes against one workgroup of 8 waves: 160 heads of 64 / 128 in f32, 500 steps 366 -> 271 us, of 128 / 64 339 ->
+// 292; 51 heads of 128 in bf16, 301 steps 108 -> 99; 2,048 heads, 128 steps 661 -> 628, in f32 1,004 -> 1,043.
+template <int KT>
+__host__ __device__ constexpr int quads_of() {
+  return KT == 8 ? 2 : 1;
+}
+template <int KT>
+inline int waves_of(int dc) {
+  return KT == 8 ? 4 : std::max(KT, tiles_of(dc));
+}
+
 // A workgroup carries one (env, head, segment) of one of the scans (blockIdx.y) through time, a wave 16 of c's columns (waves
-// past them only help to stage).  KT: 16-column tiles of a's (b's) dimension, at most the workgroup's waves: every thread brings
-// one quad of a, of b and of c.  VEC: both dimensions are multiples of four.
-// Registers for four waves a SIMD; with 8 tiles (a workgroup of 8 waves) for two, one workgroup a CU: at 128 registers S and its
-// operands spill (128 steps of 2,048 heads of 128, training: f32 1,310 -> 1,025 us, bf16 837 -> 676).  With 6 tiles in f32 for
-// three (heads of 96: 876 -> 808 us; bf16, which spills less, loses there: 507 -> 610), with 5 tiles four are best (heads of 80:
-// f32 600 us against 733 with three, bf16 412 against 558).
+// past them only help to stage).  KT: 16-column tiles of a's (b's) dimension, which its threads bring in one quad of a and of b
+// each (two with 8 tiles), and one of c.  VEC: both dimensions are multiples of four.
+// Registers for four waves a SIMD; with 8 tiles for two: at 128 registers S and its operands spill (128 steps of 2,048 heads of
+// 128, training: f32 1,310 -> 1,025 us, bf16 837 -> 676).  With 6 tiles in f32 for three (heads of 96: 876 -> 808 us; bf16, which
+// spills less, loses there: 507 -> 610), with 5 tiles four are best (heads of 80: f32 600 us against 733 with three, bf16 412
+// against 558).
 template <typename T, int KT, bool OUT, bool VEC>
 __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 3 : 4) void k_scan(Scans all) {
   typedef typename Quad<T>::M M;
@@ -274,28 +287,34 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   const int64_t t_first = s.reverse ? t_hi - 1 : t_lo, dir = s.reverse ? -1 : 1;      // step i of the scan: t_first + dir i
   const int off = s.reverse ? 0 : 1;
   const int da = s.da, dc = s.dc;
+  constexpr int AQ = quads_of<KT>();
+  const int c0 = AQ > 1 ? 16 * waves * (int)blockIdx.z : 0;      // first column of c here
 
   // this thread's quads: step and column of a and b, step and column of c
   const int arow = tid / (4 * KT), acol = 4 * (tid % (4 * KT));
   const int crow = tid / (4 * waves), ccol = 4 * (tid % (4 * waves));
   const T *pa = (const T *)s.a.p + n * s.a.sn + h * s.a.sh + (t_first + dir * arow) * s.a.st + acol;
   const T *pb = (const T *)s.b.p + n * s.b.sn + h * s.b.sh + (t_first + dir * arow) * s.b.st + acol;
-  const T *pc = (const T *)s.c.p + n * s.c.sn + h * s.c.sh + (t_first + dir * crow) * s.c.st + ccol;
+  const T *pc = (const T *)s.c.p + n * s.c.sn + h * s.c.sh + (t_first + dir * crow) * s.c.st + c0 + ccol;
   const int64_t sa = dir * s.a.st, sb = dir * s.b.st, sc = dir * s.c.st;
 
   // Every quad of a whole chunk is inside its operand: nothing to select when it is staged.  Where that is worth code of its own:
   // bf16 with the usual sizes (256 steps of 256 heads of 64: 72 -> 68 us; f32 loses 4% to the longer loop).
   constexpr bool kWhole = VEC && !M::kShare && (KT & (KT - 1)) == 0;
-  const bool whole = kWhole && waves == KT && da == 16 * KT && dc == 16 * KT;
+  const bool whole = kWhole && waves * AQ == KT && da == 16 * KT && dc - c0 >= 16 * waves;
+  constexpr int kRows = 16 / AQ;      // steps between a thread's quads of a and b
   struct Quads {
-    Quad<T> a, b, c;
+    Quad<T> a[AQ], b[AQ], c;
   };
   auto fetch = [&](Quads &q, int at, int cap) {      // the chunk of up to `cap` steps from `at` on (none past the end)
     const int m = std::min(cap, steps - at);
-    const int na = arow < m ? da - acol : 0, nc = crow < m ? dc - ccol : 0;
-    if constexpr (OUT) fetch_quad<T, VEC>(q.a, pa + at * sa, na);
-    fetch_quad<T, VEC>(q.b, pb + at * sb, na);
-    fetch_quad<T, VEC>(q.c, pc + at * sc, nc);
+#pragma unroll
+    for (int i = 0; i < AQ; ++i) {
+      const int na = arow + kRows * i < m ? da - acol : 0;
+      if constexpr (OUT) fetch_quad<T, VEC>(q.a[i], pa + (at + kRows * i) * sa, na);
+      fetch_quad<T, VEC>(q.b[i], pb + (at + kRows * i) * sb, na);
+    }
+    fetch_quad<T, VEC>(q.c, pc + at * sc, crow < m ? dc - c0 - ccol : 0);
   };
   // The flags of 64 steps a wave at a time, loaded that many steps ahead; as bits in `marks` once their turn has come.  (Loaded
   // with every chunk their addresses and conversions cost more than they look: 256 steps of 2,048 heads of 64, training, float32
@@ -314,20 +333,24 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   // the chunk's m steps into a buffer; whether b or c is not finite
   auto stage = [&](const Quads &q, int buf, int m) {
     L *A = lds(buf), *B = A + 16 * ROW, *BT = A + (OUT ? (M::kShare ? 1 : 2) * 16 * ROW : 0), *CC = BT + 16 * KT * kColStride;
-    auto put = [&](V4 a, V4 b, V4 c) {
-      if (KT >= 8 || arow < 16) {
-        if constexpr (OUT) *(V4 *)(A + arow * ROW + acol) = a;
-        if constexpr (OUT && !M::kShare) *(V4 *)(B + arow * ROW + acol) = b;
+    const bool all = kWhole && whole && m == 16;
+    const V4 c = all ? q.c.template get<VEC>() : quad_of<T, VEC>(q.c, crow < m ? dc - c0 - ccol : 0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) BT[col_at(acol, arow) + e * kColStride] = b[e];
+    for (int e = 0; e < 4; ++e) CC[col_at(ccol, crow) + e * kColStride] = c[e];
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < AQ; ++i) {
+      const int row = arow + kRows * i, na = row < m ? da - acol : 0;
+      const V4 b = all ? q.b[i].template get<VEC>() : quad_of<T, VEC>(q.b[i], na);
+      bad |= M::bad(b, c);
+      if (AQ > 1 || row < 16) {
+        if constexpr (OUT) *(V4 *)(A + row * ROW + acol) = all ? q.a[i].template get<VEC>() : quad_of<T, VEC>(q.a[i], na);
+        if constexpr (OUT && !M::kShare) *(V4 *)(B + row * ROW + acol) = b;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) BT[col_at(acol, row) + e * kColStride] = b[e];
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) CC[col_at(ccol, crow) + e * kColStride] = c[e];
-      return M::bad(b, c);
-    };
-    if (kWhole && whole && m == 16) return put(q.a.template get<true>(), q.b.template get<true>(), q.c.template get<true>());
-    const int na = arow < m ? da - acol : 0, nc = crow < m ? dc - ccol : 0;
-    return put(quad_of<T, VEC>(q.a, na), quad_of<T, VEC>(q.b, na), quad_of<T, VEC>(q.c, nc));
+    }
+    return bad;
   };
 
   Quads q = {};
@@ -346,7 +369,7 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
     }
   };
 
-  const int col = wave * 16 + x;      // this lane's column of c, of S and of the output
+  const int lcol = wave * 16 + x, col = c0 + lcol;      // this lane's column of c, of S and of the output
   f32x4 S[KT];
   {
     // state entering the segment, none: zero.  Every lane loads from an address inside it (from decay's first where there is
@@ -449,15 +472,19 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
     fetch(q, begin + chunk, next_cap);      // on its way while this chunk is worked on
     const L *A = lds(buf), *B = A + 16 * ROW, *BT = A + (OUT ? (M::kShare ? 1 : 2) * 16 * ROW : 0),
             *CC = BT + 16 * KT * kColStride;
-    const V4 C = *(const V4 *)(CC + col_at(col, 4 * g));
+    const V4 C = *(const V4 *)(CC + col_at(lcol, 4 * g));
     f32x4 P = {0.f, 0.f, 0.f, 0.f}, o = {0.f, 0.f, 0.f, 0.f};
     if constexpr (OUT) {
       if (M::kShare && wave < KT) {
-        const V4 av = *(const V4 *)(A + x * ROW + wave * 16 + 4 * g);
-        V4 bv;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bv[e] = BT[col_at(wave * 16 + 4 * g + e, x)];
-        parts[wave * 64 + lane] = M::mma(bv, av, P);
+        for (int i = 0; i < AQ; ++i) {
+          const int tile = wave + KT / AQ * i;
+          const V4 av = *(const V4 *)(A + x * ROW + tile * 16 + 4 * g);
+          V4 bv;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bv[e] = BT[col_at(tile * 16 + 4 * g + e, x)];
+          parts[tile * 64 + lane] = M::mma(bv, av, P);
+        }
       }
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
@@ -565,7 +592,7 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   float *left = nullptr;
   if (!OUT) {
     left = s.seg_state + (nh * s.segs + seg) * da * dc;
-    if (tid == 0) s.seg_coef[nh * s.segs + seg] = cut ? -1.f : (float)power_long(lam, steps);
+    if (tid == 0 && c0 == 0) s.seg_coef[nh * s.segs + seg] = cut ? -1.f : (float)power_long(lam, steps);
   } else if (s.state_out != nullptr && seg == (s.reverse ? 0 : s.segs - 1)) {
     left = s.state_out + nh * da * dc;
   }
@@ -586,7 +613,8 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
 
 template <typename T, int KT, bool OUT, bool VEC>
 void launch_k(const Scans &s, dim3 grid, hipStream_t st) {
-  const int waves = std::max(KT, tiles_of(s.s[0].dc));
+  const int waves = waves_of<KT>(s.s[0].dc);
+  if (KT == 8) grid.z = (tiles_of(s.s[0].dc) + waves - 1) / waves;
   const int bytes = lds_bytes<T, KT, OUT>(waves);
   if (bytes > 48 * 1024)      // (per device and cheap; a refusal shows at the launch)
     (void)hipFuncSetAttribute((const void *)k_scan<T, KT, OUT, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
