@@ -372,8 +372,8 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   const int lcol = wave * 16 + x, col = c0 + lcol;      // this lane's column of c, of S and of the output
   f32x4 S[KT];
   {
-    // state entering the segment, none: zero.  Every lane loads from an address inside it (from decay's first where there is
-    // none) and no value has a branch of its own: through each of those the compiler would carry all of S, and spill
+    // state entering the segment, none: zero.  Every lane loads from an address inside it and no value has a branch of its own:
+    // through each of those the compiler would carry all of S, and spill
     const int64_t size = (int64_t)da * dc;
     const float *in = s.state_in ? s.state_in + nh * size : nullptr;
     int first = 0, joins = 0;      // contributions still to be joined: segments first, first + dir, ..
@@ -387,14 +387,13 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
     }
     const bool have = OUT && in != nullptr;
     // a state from memory, in S's layout.  Four rows of a column lie side by side when it is read transposed.
-    auto load_state = [&](const float *p, bool live, f32x4 (&v)[KT]) {
+    auto load_state = [&](const float *p, f32x4 (&v)[KT]) {
       if (VEC && s.state_t) {
-        p += live ? (int64_t)std::min(col, dc - 1) * da : 0;
+        p += (int64_t)std::min(col, dc - 1) * da;
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-          if (live) __builtin_memcpy(&v[kt], p + std::min(kt * 16 + 4 * g, da - 4), 16);
+        for (int kt = 0; kt < KT; ++kt) __builtin_memcpy(&v[kt], p + std::min(kt * 16 + 4 * g, da - 4), 16);
       } else {
-        const int rs = live ? (s.state_t ? 1 : dc) : 0, cs = live ? (s.state_t ? da : 1) : 0;
+        const int rs = s.state_t ? 1 : dc, cs = s.state_t ? da : 1;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
@@ -406,10 +405,10 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) S[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
     if constexpr (OUT) {
-      load_state(have ? in : s.decay, have, S);
+      if (have) load_state(in, S);
       f32x4 u[KT];
       const float *p = s.seg_state + (nh * s.segs + first) * size, *pc = s.seg_coef + nh * s.segs + first;
-      if (joins > 0) load_state(p, true, u);
+      if (joins > 0) load_state(p, u);
       powers();                // (while those loads are on their way)
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
@@ -420,7 +419,7 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
         const float cf = pc[(int)dir * i];      // < 0: a start in that segment
         f32x4 next[KT];
         p += dir * size;
-        if (i + 1 < joins) load_state(p, true, next);
+        if (i + 1 < joins) load_state(p, next);
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
