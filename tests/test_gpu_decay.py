@@ -573,8 +573,8 @@ def test_decay_attention_in_inference_mode():
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('dk,dv', [(16, 16), (33, 40), (64, 64), (128, 100)])
 def test_decay_attention_flags_of_long_sequences(dk, dv, dtype):
-  """Enough heads that time is not cut and more steps than a workgroup takes flags of at once; some envs against the reference,
-  uint8 flags bit for bit against float32 ones."""
+  """More steps than a workgroup takes flags of at once, and enough heads that time is not cut (but for the smallest ones); some
+  envs against the reference, uint8 flags bit for bit against float32 ones."""
   a = _inputs(530, 257, 1, dk, dv, dtype=dtype, cuts=0.02, ragged=True, decay=[0.97])
   a['lengths'][:3] = torch.tensor([530, 529, 513], dtype=torch.int32)
   a['start'][[0, 63, 64, 128, 192, 255, 256, 512, 529]] = 1.0
