@@ -15,7 +15,7 @@
 //
 // One workgroup carries one (env, head, time segment), each of its waves 16 of c's columns, with the wave's columns of S in MFMA
 // accumulators from the first step to the last: 16 steps a turn, products on the 16x16 MFMA (f32 and f16 inputs: exact f32;
-// bf16 inputs: bf16, where a computed operand goes in as two or three bf16 parts).  Every accumulator is used where it lies:
+// bf16 inputs: bf16, where a computed operand goes in whole, as three bf16 parts).  Every accumulator is used where it lies:
 // lane (g = lane / 16, x = lane % 16) of a result tile holds rows 4g .. 4g + 3 of column x, which is just what the same
 // instruction takes as an operand with k = 4g + e (the sum over k may run in any order as long as both operands agree).  So the
 // pair products are made transposed (P^T = b a^T: the next product's left operand) and S multiplies from the right, with no

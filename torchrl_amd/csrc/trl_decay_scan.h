@@ -75,7 +75,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 struct Math32 {
   static constexpr bool kShare = true;
   typedef f32x4 In;
-  typedef f32x4 Part;
+  typedef f32x4 Part;      // of an operand that is computed
   static __device__ __forceinline__ f32x4 mma(const f32x4 &a, const f32x4 &b, f32x4 c) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
@@ -84,12 +84,10 @@ struct Math32 {
   static __device__ __forceinline__ Part split(const f32x4 &v) { return v; }
   static __device__ __forceinline__ f32x4 mma_right(const In &a, const Part &b, f32x4 c) { return mma(a, b, c); }
   static __device__ __forceinline__ f32x4 mma_left(const Part &a, const In &b, f32x4 c) { return mma(a, b, c); }
-  typedef f32x4 Weighed;
-  // s + b^T (w c)
-  static __device__ __forceinline__ In weigh(const In &c, const float (&w)[4]) {
+  // w c: the right operand of S + b^T (w c)
+  static __device__ __forceinline__ Part weigh(const In &c, const float (&w)[4]) {
     return f32x4{c[0] * w[0], c[1] * w[1], c[2] * w[2], c[3] * w[3]};
   }
-  static __device__ __forceinline__ f32x4 mma_state(const In &b, const In &wc, f32x4 s) { return mma(b, wc, s); }
   // whether a value is not finite (0 times it is a NaN)
   static __device__ __forceinline__ bool bad(const In &u, const In &v) {
     float d = 0.f;
@@ -99,9 +97,10 @@ struct Math32 {
   }
 };
 
-// bf16: one 16x16x16 product of the inputs as they are; what is computed in f32 goes in as a sum of bf16 parts, two of them
-// (relative error 2^-17, under a bf16 output's 2^-9) or three (2^-25) for the state, which is returned in f32.  (An infinite
-// value in f32 becomes inf + NaN: it stays not finite, but comes out as NaN.)
+// bf16: one 16x16x16 product of the inputs as they are; what is computed in f32 goes in as the sum of three bf16 parts, which
+// hold its 24 bits whole, so that a product of it is rounded as it is in f32.  (With two parts, 2^-17 of a value is lost: 0.24%
+// of a long sequence's outputs then round to the neighbour of the right bf16 value.)  An infinite value in f32 becomes
+// inf + NaN: it stays not finite, but comes out as NaN.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
 
@@ -109,9 +108,6 @@ struct Math16 {
   static constexpr bool kShare = false;
   typedef s16x4 In;
   struct Part {
-    s16x4 hi, lo;
-  };
-  struct Weighed {
     s16x4 hi, mid, lo;
   };
   static __device__ __forceinline__ f32x4 mma(const In &a, const In &b, const f32x4 &c) {
@@ -126,27 +122,20 @@ struct Math16 {
   static __device__ __forceinline__ Part split(const f32x4 &v) {
     Part p;
     p.hi = round(v);
-    p.lo = round(v - wide(p.hi));
-    return p;
-  }
-  static __device__ __forceinline__ f32x4 mma_right(const In &a, const Part &b, f32x4 c) {
-    return mma(a, b.hi, mma(a, b.lo, c));
-  }
-  static __device__ __forceinline__ f32x4 mma_left(const Part &a, const In &b, f32x4 c) {
-    return mma(a.hi, b, mma(a.lo, b, c));
-  }
-  static __device__ __forceinline__ Weighed weigh(const In &c, const float (&w)[4]) {
-    const f32x4 u = wide(c);
-    const f32x4 v = {u[0] * w[0], u[1] * w[1], u[2] * w[2], u[3] * w[3]};
-    Weighed p;
-    p.hi = round(v);
     const f32x4 r = v - wide(p.hi);
     p.mid = round(r);
     p.lo = round(r - wide(p.mid));
     return p;
   }
-  static __device__ __forceinline__ f32x4 mma_state(const In &b, const Weighed &wc, f32x4 s) {
-    return mma(b, wc.hi, mma(b, wc.mid, mma(b, wc.lo, s)));
+  static __device__ __forceinline__ f32x4 mma_right(const In &a, const Part &b, f32x4 c) {
+    return mma(a, b.hi, mma(a, b.mid, mma(a, b.lo, c)));
+  }
+  static __device__ __forceinline__ f32x4 mma_left(const Part &a, const In &b, f32x4 c) {
+    return mma(a.hi, b, mma(a.mid, b, mma(a.lo, b, c)));
+  }
+  static __device__ __forceinline__ Part weigh(const In &c, const float (&w)[4]) {
+    const f32x4 u = wide(c);
+    return split(f32x4{u[0] * w[0], u[1] * w[1], u[2] * w[2], u[3] * w[3]});
   }
   // whether an exponent is all ones: bit 15 or 31 after the addition
   static __device__ __forceinline__ uint32_t doubt(const In &v) {
@@ -529,13 +518,13 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
         }
         po += 16 * out_step;
       }
-      const typename M::Weighed wc = M::weigh(C, w_state);
+      const typename M::Part wc = M::weigh(C, w_state);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
         // (lambda^16 in two parts: its rounding would otherwise repeat in the same direction every chunk)
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[kt][r] = fmaf(S[kt][r], full_hi, S[kt][r] * full_lo);
-        S[kt] = M::mma_state(*(const V4 *)(BT + col_at(kt * 16 + x, 4 * g)), wc, S[kt]);
+        S[kt] = M::mma_right(*(const V4 *)(BT + col_at(kt * 16 + x, 4 * g)), wc, S[kt]);
       }
     } else {
       const int m = chunk;
@@ -568,10 +557,10 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
         for (int r = 0; r < 4; ++r) S[kt][r] = F == 0 ? fmaf(S[kt][r], hi, S[kt][r] * lo) : 0.f;
       // (one step alone whose own start cuts it off -- backward in time -- leaves nothing, whatever c holds)
       if (!any_bad || off == 1 || F == 0) {
-        const typename M::Weighed wc = M::weigh(C, ws);
+        const typename M::Part wc = M::weigh(C, ws);
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
-          S[kt] = M::mma_state(*(const V4 *)(BT + col_at(kt * 16 + x, 4 * g)), wc, S[kt]);
+          S[kt] = M::mma_right(*(const V4 *)(BT + col_at(kt * 16 + x, 4 * g)), wc, S[kt]);
       }
       if (any_bad) {           // rows past da: 0 times a value that is not finite
         int rows = da - 4 * g;
