@@ -199,8 +199,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd(const T *__restrict__ gy,
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        // (past the row's end g is 0, and so is every product with u)
-        const float u = (n[j][i] - m) * r;
+        // past the row's end g is 0, and u too: (0 - m) r may be infinite where every element's is finite
+        const float u = (int64_t)(j * LPR + lane) * V + (VEC ? 0 : i) < width ? (n[j][i] - m) * r : 0.f;
         // the forward's own expression: its y > 0 decides, to the bit
         const float t = ACT ? clip(fmaf(u, wv[j][i], bv[j][i]), g[j][i]) : g[j][i];
         const float h = t * wv[j][i];
