@@ -27,6 +27,7 @@
 //
 // Values that are not finite stay where the recurrence puts them: masks are selections, never products with zero -- except
 // of b's and c's steps inside a chunk, so a chunk whose b or c holds an infinity or a NaN is taken one step at a time.
+// An infinite state stays infinite, of its sign, for ever (bf16: its products come out as NaN).
 #include <algorithm>
 #include <cmath>
 

@@ -46,24 +46,42 @@ constexpr int kJoinInside = 8;
 
 inline int tiles_of(int dim) { return (dim + 15) / 16; }
 
-// lambda^n in double, n < 32: each power is rounded to f32 once
+// lambda^n in double, n < 32: each power is rounded to f32 once.  Not zero unless lambda is
 __device__ __forceinline__ double power(double lam, int n) {
+  const bool zero = lam == 0.0;
   double p = 1.0;
 #pragma unroll
   for (int b = 0; b < 5; ++b) {
     if ((n >> b) & 1) p *= lam;
     lam *= lam;
   }
-  return p;
+  return p == 0.0 && !zero ? __DBL_MIN__ : p;
 }
 
 __device__ __forceinline__ double power_long(double lam, int64_t n) {
+  const bool zero = lam == 0.0;
   double p = 1.0;
   for (; n > 0; n >>= 1) {
     if (n & 1) p *= lam;
     lam *= lam;
   }
-  return p;
+  return p == 0.0 && !zero ? __DBL_MIN__ : p;
+}
+
+// Rounded to f32, and not to zero: what the state is multiplied with, whose infinities stay infinite for ever
+__device__ __forceinline__ float not_to_zero(double p) {
+  const float f = (float)p;
+  return f == 0.f && p != 0.0 ? copysignf(__FLT_DENORM_MIN__, f) : f;
+}
+
+// A power of lambda in two parts, for the state (its rounding alone would repeat in the same direction every chunk).  The large
+// part is rounded down and the small one above zero, if only by the smallest float: hi s + lo s of an infinite s is s then,
+// where parts of different signs, or a small part of zero, would make it a NaN.
+__device__ __forceinline__ void two_parts(double p, float &hi, float &lo) {
+  hi = not_to_zero(p);
+  if ((double)hi > p && hi > __FLT_DENORM_MIN__) hi = __int_as_float(__float_as_int(hi) - 1);
+  lo = (float)(p - (double)hi);
+  if (p > 0.0) lo = fmaxf(lo, __FLT_DENORM_MIN__);
 }
 
 namespace {
@@ -255,7 +273,7 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   __shared__ int bad_flag[2][8];
   __shared__ uint64_t marks[2][8];
-  __shared__ float pw[48], pw_lo[32];
+  __shared__ float pw[48], pw_hi[32], pw_lo[32];
   const Scan &s = all.s[blockIdx.y];
   const int tid = threadIdx.x, waves = blockDim.x >> 6;
   const int lane = tid & 63, x = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -352,8 +370,8 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   auto powers = [&]() {
     if (tid < 32) {
       const double p = power(lam, tid);
-      pw[16 + tid] = (float)p;
-      pw_lo[tid] = (float)(p - (double)(float)p);
+      pw[16 + tid] = not_to_zero(p);
+      two_parts(p, pw_hi[tid], pw_lo[tid]);
       if (tid < 16) pw[tid] = 0.f;
     }
   };
@@ -429,10 +447,10 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     w_intra[r] = pw[16 + x - 4 * g - r] * s.s_intra;
-    w_inter[r] = pw[16 + off + 4 * g + r] * s.s_inter;
+    w_inter[r] = not_to_zero((double)pw[16 + off + 4 * g + r] * s.s_inter);
     w_state[r] = pw[32 - off - 4 * g - r] * s.s_state;
   }
-  const float full_hi = pw[32], full_lo = pw_lo[16];
+  const float full_hi = pw_hi[16], full_lo = pw_lo[16];
 
   const int64_t out_step = dir * heads * dc;
   T *po = OUT ? (T *)s.out + ((t_first + dir * 4 * g) * heads + nh) * dc + col : nullptr;      // step 4 g of the chunk
@@ -521,7 +539,6 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
       const typename M::Part wc = M::weigh(C, w_state);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        // (lambda^16 in two parts: its rounding would otherwise repeat in the same direction every chunk)
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[kt][r] = fmaf(S[kt][r], full_hi, S[kt][r] * full_lo);
         S[kt] = M::mma_right(*(const V4 *)(BT + col_at(kt * 16 + x, 4 * g)), wc, S[kt]);
@@ -550,7 +567,7 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         ws[e] = (F & ~((1u << (4 * g + e + off)) - 1)) == 0 ? pw[16 + m - off - 4 * g - e] * s.s_state : 0.f;
-      const float hi = pw[16 + m], lo = pw_lo[m];
+      const float hi = pw_hi[m], lo = pw_lo[m];
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -580,7 +597,7 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   float *left = nullptr;
   if (!OUT) {
     left = s.seg_state + (nh * s.segs + seg) * da * dc;
-    if (tid == 0 && c0 == 0) s.seg_coef[nh * s.segs + seg] = cut ? -1.f : (float)power_long(lam, steps);
+    if (tid == 0 && c0 == 0) s.seg_coef[nh * s.segs + seg] = cut ? -1.f : not_to_zero(power_long(lam, steps));
   } else if (s.state_out != nullptr && seg == (s.reverse ? 0 : s.segs - 1)) {
     left = s.state_out + nh * da * dc;
   }
