@@ -8,6 +8,7 @@
 #include <torch/extension.h>
 
 #include <cstring>
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -78,6 +79,13 @@ variable_list first_order(variable_list grads) {
 
 bool wants(const Tensor &t) { return t.defined() && t.requires_grad(); }
 
+// There are no forward-mode derivatives: an input that carries a tangent is an error (and not a result without one)
+void no_tangents(const char *fn, std::initializer_list<Tensor> inputs) {
+  for (const Tensor &t : inputs)
+    if (t.defined() && t._fw_grad(/*level=*/0).defined())
+      throw std::runtime_error(std::string(fn) + " has no forward-mode derivative");
+}
+
 // ---------------------------------------------------------------------------------------------- layer norm
 // (each buffer is of one call alone, so two streams or two captured graphs never share one)
 Tensor norm_run(const Tensor &x, const Tensor &w, const Tensor &b, double eps, int64_t act, int64_t stream, Tensor *stats) {
@@ -124,6 +132,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 
 Tensor layer_norm(const Tensor &x, const Maybe &w, const Maybe &b, double eps, int64_t act, int64_t stream) {
+  no_tangents("layer_norm", {x, get(w), get(b)});
   if (at::GradMode::is_enabled() && (wants(x) || wants(get(w)) || wants(get(b))))
     return LayerNorm::apply(x, w, b, eps, act, stream);
   return norm_run(x.contiguous(), get(w), get(b), eps, act, stream, nullptr);
@@ -164,6 +173,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 
 Tensor dropout(const Tensor &x, const Maybe &residual, double p, uint64_t seed, uint64_t call, const Maybe &call_d,
                int64_t stream) {
+  no_tangents("dropout", {x, get(residual)});
   if (at::GradMode::is_enabled() && (wants(x) || wants(get(residual))))
     return Dropout::apply(x, residual, p, (int64_t)seed, (int64_t)call, call_d, stream);
   return dropout_run(x.contiguous(), residual ? residual->contiguous() : Tensor(), p, seed, call, get(call_d), stream);
@@ -223,6 +233,7 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
 std::vector<Tensor> decay_attention(const Tensor &q, const Tensor &k, const Tensor &v, const Maybe &state, const Tensor &decay,
                                     const Maybe &start, const Maybe &lengths, int64_t start_code, double scale,
                                     int64_t stream) {
+  no_tangents("decay_attention", {q, k, v, get(state), decay});
   if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v) || wants(get(state))))
     return DecayAttention::apply(q, k, v, state, decay, start, lengths, start_code, scale, stream);
   return decay_run(q, k, v, get(state), decay, get(start), get(lengths), start_code, scale, stream);
@@ -231,6 +242,7 @@ std::vector<Tensor> decay_attention(const Tensor &q, const Tensor &k, const Tens
 // (no gradients; out_state may be state)
 std::vector<Tensor> decay_step(const Tensor &q0, const Tensor &k0, const Tensor &v0, const Tensor &decay, const Maybe &start,
                                int64_t start_code, const Tensor &state, const Maybe &out_state, double scale, int64_t stream) {
+  no_tangents("decay_attention_step", {q0, k0, v0, state, decay});
   const Tensor q = q0.contiguous(), k = k0.contiguous(), v = v0.contiguous();
   Tensor out = at::empty(v.sizes(), v.options()), next = out_state ? *out_state : at::empty(state.sizes(), state.options());
   check(api.decay_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), fptr(decay), ptr(get(start)), (int32_t)start_code, fptr(state),

@@ -4,7 +4,8 @@ Every function here takes device tensors and enqueues kernels on torch's current
 There is no CPU implementation behind any of them: a CPU tensor raises TrlError.
 The loss functions are autograd Functions whose forward runs the fused kernel (loss AND
 its backward seeds in one pass) and whose backward only scales the saved seeds.  Layer norm, dropout and
-decay attention have their graph nodes in native code (csrc/trl_autograd.cpp); their arguments are checked here.
+decay attention have their graph nodes in native code (csrc/trl_autograd.cpp); their arguments are checked here.  They have
+first derivatives in reverse mode: forward mode and second derivatives are refused.
 
 Everything here can be captured into a HIP graph.  As with any of torch's operators, capture a backward pass only while no
 eager graph of the same leaves is alive: torch keeps a leaf's gradient accumulator, and the stream that it was made on, for as
