@@ -654,6 +654,8 @@ def next_call(counter):
   _lib.require_device(counter, 'next_call: counter')
   if counter.dtype != torch.int64 or counter.numel() != 1:
     raise ValueError('next_call: counter must be an int64 tensor of one element')
+  if not counter.is_inference():      # (a graph that saved it as it was refuses its backward pass)
+    torch.autograd.graph.increment_version(counter)
   call = torch.empty(1, dtype=torch.int64, device=counter.device)
   with _lib.device_guard(counter.device):
     _lib.check(_lib.lib().trl_next_call(counter.data_ptr(), call.data_ptr(), _lib.stream_ptr(counter.device)))
