@@ -102,7 +102,7 @@ class Dropout(nn.Module):
   from and raises on the stream, so a step captured into a HIP graph gets a new mask at every replay, and under
   the same seed a checkpoint carries on where it was taken.  seed: by default torch.initial_seed() mixed with a number that differs for every layer of
   the process and every rank.  In eval mode x passes through.  A forward pass that is run again for its gradients (activation
-  checkpointing) would draw another mask: give functional.dropout the call number there."""
+  checkpointing) would draw another mask and is refused: give functional.dropout the call number there."""
 
   def __init__(self, p, seed=None):
     super().__init__()

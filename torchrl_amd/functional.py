@@ -650,7 +650,11 @@ def dropout(x, p, seed, call, residual=None):
 
 def next_call(counter):
   """A fresh device tensor holding the value of `counter` (int64, one element, on the device), which goes up by one: the
-  call number of one dropout call, drawn on the stream -- so also at every replay of a captured graph."""
+  call number of one dropout call, drawn on the stream -- so also at every replay of a captured graph.  Refused inside a
+  backward pass: what is run again there (activation checkpointing) has to have the number of the first time."""
+  if torch._C._current_graph_task_id() != -1:
+    raise RuntimeError('next_call: a forward pass run again for its gradients (activation checkpointing) would draw another '
+                       'number, and dropout another mask: draw it outside and give functional.dropout that')
   _lib.require_device(counter, 'next_call: counter')
   if counter.dtype != torch.int64 or counter.numel() != 1:
     raise ValueError('next_call: counter must be an int64 tensor of one element')
