@@ -632,7 +632,7 @@ int trl_layer_norm_bwd(const void *gy, const void *x, const float *weight, const
                        const float *rstd, int64_t rows, int64_t width, int32_t dtype, int32_t act, void *dx, float *dweight,
                        float *dbias, void *workspace, void *stream);
 
-/* y[i] = (residual ? residual[i] : 0) + (kept(i) ? x[i] / (1 - p) : 0) over n elements (n < 2^40), 0 <= p < 1.  Element i is
+/* y[i] = (residual ? residual[i] : 0) + (kept(i) ? x[i] / (1 - p) : 0) over n elements (n < 2^40), 0 <= p < 1 - 2^-33.  Element i is
  * kept when word i % 4 of Philox-4x32-10 -- key = seed, counter = (call low, call high, (i / 4) low, (i / 4) high | 2^31) --
  * is at least round(p 2^32); no mask is stored, the gradient of x is the same call on dL/dy (residual NULL).  `call` is read
  * from *call_d (device) when that is not NULL: a captured graph then draws a new mask at every replay. */

@@ -106,8 +106,8 @@ class Dropout(nn.Module):
 
   def __init__(self, p, seed=None):
     super().__init__()
-    if not 0.0 <= p < 1.0:
-      raise ValueError('Dropout: p must be in [0, 1), got %r' % (p,))
+    if not 0.0 <= p < _F.MAX_DROPOUT:
+      raise ValueError('Dropout: p must be in [0, 1 - 2^-33), got %r' % (p,))
     self.p = float(p)
     self._given = seed
     self._rng = _F.ActRng(seed)

@@ -496,7 +496,7 @@ extern "C" int trl_layer_norm_bwd(const void *gy, const void *x, const float *we
 
 // ---------------------------------------------------------------------------------------------- dropout
 // Element i of call c is kept when word i % 4 of Philox-4x32-10 with key = seed and counter = (c, i / 4 with its top bit set)
-// is at least p 2^32: the mask of a call is a function of (seed, c, i) alone, so the backward pass makes it again instead of
+// is at least round(p 2^32): the mask of a call is a function of (seed, c, i) alone, so the backward pass makes it again instead of
 // reading it, and a call on a part of the memory or on another grid keeps the same elements.  (The top bit keeps the
 // counters apart from those of the exploration draws, csrc/trl_act.hip, under an equal seed.)
 // The generator costs 18 32 x 32 -> 64 bit products a lane for four elements (two of its 20 are the same for a whole wave).  In
@@ -576,12 +576,12 @@ extern "C" int trl_dropout(const void *x, const void *residual, int64_t n, int32
   const char *fn = "trl_dropout";
   TRL_REQUIRE(trl_float_dtype(dtype), "%s: dtype %d is not f32, bf16 or f16", fn, (int)dtype);
   TRL_REQUIRE(n >= 0 && n < ((int64_t)1 << 40), "%s: bad length %lld", fn, (long long)n);
-  TRL_REQUIRE(p >= 0.0 && p < 1.0, "%s: p must be in [0, 1)", fn);
+  const double t = p * 4294967296.0 + 0.5;      // (at 2^32 no word would be large enough)
+  TRL_REQUIRE(p >= 0.0 && t < 4294967296.0, "%s: p must be in [0, 1 - 2^-33)", fn);
   if (n == 0) return TRL_OK;
   TRL_REQUIRE(x != nullptr && y != nullptr, "%s: null pointer", fn);
   const hipStream_t st = (hipStream_t)stream;
-  const double t = p * 4294967296.0 + 0.5;
-  const uint32_t threshold = t >= 4294967295.0 ? 0xFFFFFFFFu : (uint32_t)t;
+  const uint32_t threshold = (uint32_t)t;
   const float scale = (float)(1.0 / (1.0 - p));
   const int grid = (int)std::min<int64_t>(trl_cdiv(n, (int64_t)kThreads * (16 / elem_bytes(dtype))), 2048);
   TRL_FOR_DTYPE(dtype, {

@@ -575,6 +575,7 @@ def linear_u8(x, weight, bias, relu=False):
 
 # ------------------------------------------------------------------------------ layer norm, dropout
 LAYER_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+MAX_DROPOUT = 1.0 - 2.0 ** -33      # round(p 2^32) is a 32-bit word below it
 
 
 def _layer_dtype(t, what):
@@ -626,11 +627,12 @@ def dropout(x, p, seed, call, residual=None):
   backward pass makes it again.  A dropped element gives 0 whatever it held.  call: a number, or a device int64 tensor of
   one element (next_call) that is read when the kernel runs -- what a captured graph needs to draw a new mask at
   every replay.  Every use within one call number gets the same mask: number the calls, or seed the layers, apart.
-  x, residual: float32, bfloat16 or float16, equal shapes and types; 0 <= p < 1."""
+  x, residual: float32, bfloat16 or float16, equal shapes and types; 0 <= p < 1 - 2^-33 (above it no word is
+  large enough)."""
   _layer_dtype(x, 'dropout: x')
   p = float(p)
-  if not 0.0 <= p < 1.0:
-    raise ValueError('dropout: p must be in [0, 1), got %r' % p)
+  if not 0.0 <= p < MAX_DROPOUT:
+    raise ValueError('dropout: p must be in [0, 1 - 2^-33), got %r' % p)
   call_d = None
   if torch.is_tensor(call):
     _beside(call, x, 'dropout: call')
