@@ -83,14 +83,16 @@ class SkinnyLinear(nn.Linear):
 
 class LayerNorm(nn.LayerNorm):
   """nn.LayerNorm over the last dimension (same parameters, same values) on the HIP layer (csrc/trl_norm.hip) for float32,
-  bfloat16 and float16 device batches; `relu=True` applies the ReLU behind it in the same launch.  Anything else, and
-  config.fused_mlp = False, takes torch's."""
+  bfloat16 and float16 device batches; `relu=True` applies the ReLU behind it in the same launch.  Under autocast the
+  result is float32, as nn.LayerNorm's is.  Anything else, and config.fused_mlp = False, takes torch's."""
 
   def __init__(self, width, eps=1e-5):
     super().__init__(int(width), eps=eps)
 
   def forward(self, x, relu=False):
     if x.is_cuda and x.dtype in _F.LAYER_DTYPES and _fused_mlp_enabled():
+      if torch.is_autocast_enabled('cuda'):
+        x = x.float()
       return _F.layer_norm(x, self.weight, self.bias, self.eps, relu=relu)
     x = super().forward(x)
     return torch.relu(x) if relu else x
