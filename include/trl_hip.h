@@ -620,6 +620,8 @@ int trl_act_ou_noise(const float *actor_out, int64_t n, int32_t A, const float *
  * The normalising and the regularising layer of a Linear / ReLU stack.  No counterpart in the reference (its stacks are
  * Linear + ReLU, models.py:6-147).  x, y, gy, dx: dense [rows, width] of `dtype` (TRL_F32, TRL_BF16, TRL_F16), any alignment
  * of the element; weight, bias, mean, rstd and their gradients f32.  1 <= width < 2^24, rows * width < 2^40; rows may be 0.
+ * Outputs overlap no input.  Statistics are f32 sums: a row whose sum, or whose squared distances from the mean, pass the
+ * largest f32 has what an infinity there makes of it.
  *
  * fwd: y = (x - m) r * weight + bias per row, m = mean, r = 1 / sqrt(variance + eps), act = 1: max(y, 0) (a NaN stays one).
  *   weight / bias NULL: ones / zeros.  mean, rstd [rows] (NULL: not written) are what bwd takes.
@@ -649,7 +651,9 @@ int trl_next_call(int64_t *counter, int64_t *call, void *stream);
  * with strides[9] = (t, n, h) of q, of k and of v in elements (a dimension may have stride 0; the last one is dense);
  * out [T, N, H, dv] dense; states [N, H, dk, dv] f32 dense; decay [H] f32, each in [0, 1]; start [T, N] dense, start_dtype
  * TRL_F32 or TRL_U8, not zero = the step does not see the ones before it; lengths [N] int32, cut to [0, T], or NULL.
- * 1 <= dk, dv <= 128, T < 2^30, N * H < 2^22.  Sums and states in f32.
+ * 1 <= dk, dv <= 128, T < 2^30, N * H < 2^22.  Sums and states in f32; bf16 inputs are multiplied as they are, what is
+ * computed with its 24 bits.  An infinite state stays infinite (its products with bf16 inputs are NaN).  Outputs overlap no input,
+ * except in step.
  * bwd: gy [T, N, H, dv] dense, gstate (gradient of state_out) [N, H, dk, dv] or NULL; dq, dk_out, dv_out dense; dstate
  *   (gradient of state_in) or NULL.  Zero at and past lengths[n].
  * step: the same for one step, q, k [N, H, dk], v [N, H, dv], start [N]; state_out may be state_in.

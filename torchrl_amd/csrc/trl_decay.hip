@@ -87,8 +87,9 @@ __global__ __launch_bounds__(kThreads) void k_join(Scans all, int64_t heads, int
 }
 
 // One step: a workgroup per (env, head); LC lanes hold four columns each (the fewest that hold a row, so that a wave's access
-// is whole rows), the others share out the rows.  Bound by the state's one read and one write: 4,096 envs of 4 heads of 64 x 64
-// take 105 us, 5.1 TB/s; one env 3.2 us.
+// is whole rows), the others share out the rows.  Heads of 64 x 64 are bound by the state's one read and one write: 4,096 envs of
+// 4 of them take 105 us, 5.1 TB/s, 1,024 of 128 x 128 113 us, 4.7; one env 3.2 us.  Small heads leave threads without work, 64 of
+// 256 have some at 16 x 16 and 16 at 8 x 8: 65,536 envs of 4 heads of 16 x 16 347 us, 1.7 TB/s, 262,144 of 8 x 8 1,167, 0.6.
 template <typename T, int LC>
 __global__ __launch_bounds__(kThreads) void k_step(const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
                                                    const float *__restrict__ decay, const void *__restrict__ start,
@@ -133,12 +134,12 @@ __global__ __launch_bounds__(kThreads) void k_step(const T *__restrict__ q, cons
 
 // Time segments: as many as bring the launch to 2,048 waves (two a SIMD; a workgroup has one for 16 columns of a head), each of
 // at least 64 steps, no more than sqrt(T) of them, and none where that makes fewer than three.  Training passes, us:
-//  * waves, not workgroups: 128 heads of 128 in bf16, 400 steps: 2,048 waves 178, 4,096 231; 128 heads of 32 in f32, 400
+//  * waves, not workgroups: 128 heads of 128 in bf16, 400 steps: 2,048 waves 185, 4,096 243; 128 heads of 32 in f32, 400
 //    steps: 1,536 waves 57, 1,024 65, 256 82.
 //  * two halves take as long as the whole, since a contribution costs most of a segment's work again: 256 heads of 64 in f32, 256
 //    steps: two segments 119, one 97; 128 heads, 128 steps: 57 and 49; but 128 heads, 1,024 steps: four 210, one 252.
-//  * shorter ones are mostly start and join, longer ones a longer chain: 64 heads of 64 in bf16, 500 steps: at least 64 steps 72,
-//    128 steps 81; 128 heads of 64, 128 steps: at least 32 steps 61, 64 steps 49.
+//  * shorter ones are mostly start and join, longer ones a longer chain: 64 heads of 64 in bf16, 500 steps: at least 64 steps 75,
+//    128 steps 85, 111 heads of 48 / 80, 333 steps: 113 and 130; 128 heads of 64, 128 steps: at least 32 steps 61, 64 steps 49.
 //  * the join walks the segments one after another: one head of 16 in f32, 131,072 steps: 362 segments 176, 2,048 485, 128 237;
 //    32,768 steps: 181 segments 95, 512 143.
 void segments(int64_t T, int64_t heads, int32_t dk, int32_t dv, int *segs, int *seg_len) {

@@ -40,7 +40,7 @@ void launch_f16(const Scans &all, int count, bool out, hipStream_t st);
 
 // up to so many segments a workgroup joins the contributions before its own by itself: 2 us at 8 of them, against 7 us and a
 // launch for the join of all; beyond, what all workgroups read grows with the square of the segments.  (Training passes: 64 heads
-// of 64 in bf16, 500 steps in 7 segments: 71 us, joined by the launch 75; 8 heads of 128 in f32, 1,024 steps in 16 segments: by
+// of 64 in bf16, 500 steps in 7 segments: 75 us, joined by the launch 81; 8 heads of 128 in f32, 1,024 steps in 16 segments: by
 // the launch 101, by the workgroups 141.)
 constexpr int kJoinInside = 8;
 
@@ -246,8 +246,8 @@ constexpr int lds_bytes(int waves) {
 
 // Waves of a workgroup, and quads of a (and b) that each of its threads brings.  With 8 tiles of a's dimension a workgroup of 4
 // waves takes 64 of c's columns (blockIdx.z), so that two of them share a CU and one works while the other starts, ends or waits.
-// Training passes against one workgroup of 8 waves: 160 heads of 64 / 128 in f32, 500 steps 366 -> 271 us, of 128 / 64 339 ->
-// 292; 51 heads of 128 in bf16, 301 steps 108 -> 99; 2,048 heads, 128 steps 661 -> 628, in f32 1,004 -> 1,043.
+// Training passes against one workgroup of 8 waves: 160 heads of 64 / 128 in f32, 500 steps 369 -> 276 us, of 128 / 64 345 ->
+// 299; 51 heads of 128 in bf16, 301 steps 120 -> 109; 2,048 heads, 128 steps 823 -> 764, in f32 1,028 -> 1,074.
 template <int KT>
 __host__ __device__ constexpr int quads_of() {
   return KT == 8 ? 2 : 1;
@@ -261,9 +261,10 @@ inline int waves_of(int dc) {
 // past them only help to stage).  KT: 16-column tiles of a's (b's) dimension, which its threads bring in one quad of a and of b
 // each (two with 8 tiles), and one of c.  VEC: both dimensions are multiples of four.
 // Registers for four waves a SIMD; with 8 tiles for two: at 128 registers S and its operands spill (128 steps of 2,048 heads of
-// 128, training: f32 1,310 -> 1,025 us, bf16 837 -> 676).  With 6 tiles in f32 for three (heads of 96: 876 -> 808 us; bf16, which
-// spills less, loses there: 507 -> 610), with 5 tiles four are best (heads of 80: f32 600 us against 733 with three, bf16 412
-// against 558).
+// 128, training: f32 2,098 -> 1,072 us, bf16 1,116 -> 763).  With 6 tiles in f32 for three (heads of 96: 876 -> 815 us; bf16 loses
+// there: 691 -> 702), with 5 tiles four are best (heads of 80: f32 608 us against 714 with three, bf16 540 against 628).
+// At these bounds 3, 4, 5 and 6 tiles keep 28, 60, 160 and 20 B a lane in scratch in f32, 4, 5 and 6 tiles 32, 128 and 240 B in
+// bf16 (VEC; f16 like f32 or less): most of it values of the prologue and the epilogue, kept over the loop.
 template <typename T, int KT, bool OUT, bool VEC>
 __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 3 : 4) void k_scan(Scans all) {
   typedef typename Quad<T>::M M;
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(512, KT == 8 ? 2 : KT == 6 && Quad<T>::M::kShare ? 
   const int64_t sa = dir * s.a.st, sb = dir * s.b.st, sc = dir * s.c.st;
 
   // Every quad of a whole chunk is inside its operand: nothing to select when it is staged.  Where that is worth code of its own:
-  // bf16 with the usual sizes (256 steps of 256 heads of 64: 72 -> 68 us; f32 loses 4% to the longer loop).
+  // bf16 with the usual sizes (128 steps of 2,048 heads of 128: 777 -> 763 us; f32 loses 4% to the longer loop).
   constexpr bool kWhole = VEC && !M::kShare && (KT & (KT - 1)) == 0;
   const bool whole = kWhole && waves * AQ == KT && da == 16 * KT && dc - c0 >= 16 * waves;
   constexpr int kRows = 16 / AQ;      // steps between a thread's quads of a and b

@@ -6,13 +6,17 @@
 //     y = n w + b  (then max(y, 0) with act);    with g = gy (0 where act clipped) and h = g w:
 //     dx = r (h - mean(h) - n mean(h n)),   dw = sum over rows of g n,   db = sum over rows of g.
 // Both directions are bound by memory: a row lives in the registers of LPR lanes from its one read to its one write, the
-// mean and the centred second moment are two sums over those registers (no E[x^2] - m^2 cancellation).
+// mean and the centred second moment are two sums over those registers (no E[x^2] - m^2 cancellation).  (The backward pass of
+// 16-bit rows of 8,193 to 16,384 elements has more than the registers hold: up to 800 B a lane of it are in scratch.)
 // The weight's and the bias's gradients need a sum over all rows: every lane owns fixed columns, adds them up over the rows
 // its workgroup walks, the workgroup's lane groups are added in order, and a second launch adds the workgroups' partial sums
 // in order: no atomics, the same bits every run.
 // Measured: 1M x 64 f32 forward 96 us (5.6 TB/s), backward 160 us (5.0 TB/s) + 5 us for the join of the parts; 16k x 1024 bf16
 // 13.0, 21.8 and 4.5 us (the data stay in the last-level cache); 10007 x 257 f32 8.8, 10.0 and 4.2; 16 x 64 1.6 us.  A training
-// call on small data is bound by the host and the graph engine (46 us and more), not by these.
+// call on small data is bound by the host and the graph engine (40 us and more), not by these.
+// Rows that are not whole slots cost more, since each slot carries code for single elements beside its 16 B access: a training
+// pass over 256k x 257 takes 334 us in f32 (3.2 TB/s; 260 columns 296) and 310 in bf16 (1.7 TB/s; 264 columns 149).  16-bit
+// rows of many slots: 4,096 x 8,192 bf16 125 us (2.2 TB/s), 4,096 x 12,000 200 (2.0).
 #include <algorithm>
 
 #include "trl_io.h"
