@@ -253,7 +253,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd(const T *__restrict__ gy,
     }
 }
 
-// Rows wider than the registers of a workgroup (more than 8,192 f32 or 16,384 elements of 16 bits): one workgroup a row, the
+// Rows of more slots than shape_of has lanes for (more than 8,192 f32 or 16,384 elements of 16 bits): one workgroup a row, the
 // row read once per pass (from L2 after the first).  Correct at any width; not tuned: no network here is that wide.
 template <typename T, bool ACT>
 __global__ __launch_bounds__(kThreads) void k_norm_fwd_wide(const T *__restrict__ x, const float *__restrict__ w,
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(1024) void k_norm_fold(const float *__restrict__ pa
 }
 
 // Lanes a row and 16 B slots a lane by the number of slots of a row: the fewest lanes that hold it in few slots, so that a
-// wave works on several narrow rows at once and up to 256 slots need no barrier; 0 = wider than a workgroup's registers.
+// wave works on several narrow rows at once and up to 256 slots need no barrier; 0 = more slots than it has lanes for.
 // Training passes against a wave for every row of at most 64 slots and a workgroup for wider ones: 1M x 32 f32 134 us against
 // 384, 1M x 64 263 / 423, 256k x 128 bf16 62 / 117, 16k x 512 f32 37 / 47, 64k x 1024 bf16 139 / 233, 10007 x 257 f32 26 / 45;
 // even only for 16k x 1024 f32 (66 / 64).
